@@ -5,7 +5,7 @@ library is missing or cannot be loaded the import of the package fails with the 
 """
 import ctypes
 import os
-from ctypes import (POINTER, Structure, c_char_p, c_double, c_float, c_int, c_long, c_size_t, c_void_p)
+from ctypes import (POINTER, Structure, c_char_p, c_double, c_float, c_int, c_long, c_longlong, c_size_t, c_void_p)
 
 _PKG = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_PKG, "libdeepracin.so")
@@ -102,6 +102,18 @@ _SIGS = {
     "dR_getScratchFloats": (c_size_t, [c_void_p]),
     "dR_b200_version": (c_char_p, []),
     # operator-level kernel ABI (include/dR_kernels.h)
+    "dRk_fp8_fc_supported": (c_int, [c_int, c_int, c_int]),
+    "dRk_fp8_fc_packed_bytes": (c_size_t, [c_int, c_int]),
+    "dRk_fp8_fc_scratch_bytes": (c_size_t, [c_int, c_int, c_int]),
+    "dRk_fp8_fc_pack_weights": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int]),
+    "dRk_fp8_fc_pack_codes": (c_int, [c_void_p, c_void_p, c_longlong, c_void_p, c_void_p, c_int, c_int]),
+    "dRk_fp8_fc_unpack_weights": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int]),
+    "dRk_fp8_fc_plan": (c_void_p, [c_void_p, c_int, c_longlong, c_void_p, c_void_p, c_void_p, c_int, c_longlong, c_void_p,
+                                   c_int, c_int, c_int, c_int, c_void_p]),
+    "dRk_fp8_fc_run": (c_int, [c_void_p, c_void_p]),
+    "dRk_fp8_fc_free": (None, [c_void_p]),
+    "dRk_logprobs": (c_int, [c_void_p, c_void_p, c_int, c_longlong, c_int, c_int, c_float, c_void_p, c_int, c_void_p, c_void_p,
+                             c_int, c_void_p, c_void_p]),
     "dRk_launch_count": (c_long, []),
     "dRk_launch_count_reset": (None, []),
 }

@@ -2,6 +2,7 @@
 #pragma once
 #include <cuda_runtime.h>
 #include <float.h>
+#include <stdio.h>
 #include <stdint.h>
 #include "dR_kernels.h"
 
@@ -52,4 +53,31 @@ static inline cudaError_t drk_launch_dep(void (*kernel)(KArgs...), dim3 grid, di
     cfg.attrs = attr;
     cfg.numAttrs = drk_dep_launch_enabled() ? 1 : 0;
     return cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
+}
+
+/* Device that is current if the stream belongs to it; negative, with a message that begins with `who`, if there is none (-5) or
+ * if the stream or what `want` >= 0 stands for belongs to another one (-6).  A stream that is being captured cannot be asked
+ * (the question would end the capture); a launch into another device's fails by itself. */
+static inline int drk_stream_device(const char *who, dRk_stream stream, int want)
+{
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) { (void)cudaGetLastError(); fprintf(stderr, "%s: no CUDA device\n", who); return -5; }
+    int sdev = dev;
+    cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
+    if (cudaStreamIsCapturing(drk_stream(stream), &capturing) != cudaSuccess) { (void)cudaGetLastError(); capturing = cudaStreamCaptureStatusActive; }
+    if (capturing == cudaStreamCaptureStatusNone && cudaStreamGetDevice(drk_stream(stream), &sdev) != cudaSuccess) { (void)cudaGetLastError(); sdev = dev; }
+    if (sdev != dev || (want >= 0 && want != dev)) {
+        fprintf(stderr, "%s: device %d is current, the stream belongs to device %d%s\n", who, dev, sdev,
+                want >= 0 && want != dev ? " and the plan to another one" : "");
+        return -6;
+    }
+    return dev;
+}
+
+/* outcome of a launch: counted and 0, or its error, taken off the runtime's record */
+static inline int drk_launched(cudaError_t e)
+{
+    if (e != cudaSuccess) { (void)cudaGetLastError(); return (int)e; }
+    DRK_COUNT_LAUNCH();
+    return 0;
 }

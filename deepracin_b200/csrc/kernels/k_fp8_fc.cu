@@ -1,0 +1,335 @@
+/*
+ * Fully connected layer with operands in 8-bit floating point (e4m3), a scale for each block of 128:
+ *
+ *   out[r][o] = act(bias[o] + sum_b sx[b][r] * sw[o / 128][b] * sum_{k in block b} qx[r][k] * qw[o][k])
+ *
+ * Weights carry one float scale per 128 x 128 block, each row of the input one per block of 128 values, taken when the
+ * layer runs: A = max(largest |x| of the block, 2^-96), qx = e4m3(x * (448 / A)), sx = A / 448 (all in 32 bits, codes
+ * rounded to nearest even).  The sums of a block and over the blocks are held in 32 bits.
+ *
+ * Packed weights: [ceil(Nout/128)][ceil(Nin/128)] blocks of 128 rows (outputs) x 128 bytes (inputs), zero behind the edges,
+ * then their scales as floats in the same order.  A block is one contiguous 16 KiB run, so a weight stream reads DRAM in order.
+ */
+#include <math.h>
+#include <stdio.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+#include "k_common.cuh"
+
+#define FP8_BLOCK 128
+#define FP8_BLOCK_BYTES (FP8_BLOCK * FP8_BLOCK)
+#define FP8_MAX 448.0f
+#define FP8_FLOOR 0x1p-96f      /* smallest block maximum a scale is made from: 448 / A stays finite */
+
+static int fp8_blocks(int n) { return (int)(((long long)n + FP8_BLOCK - 1) / FP8_BLOCK); }
+
+template <typename T> __device__ __forceinline__ float fp8_load(const T *p);
+template <> __device__ __forceinline__ float fp8_load(const float *p) { return *p; }
+template <> __device__ __forceinline__ float fp8_load(const __nv_bfloat16 *p) { return __bfloat162float(*p); }
+template <> __device__ __forceinline__ float fp8_load(const __half *p) { return __half2float(*p); }
+template <typename T> __device__ __forceinline__ T fp8_store(float v);
+template <> __device__ __forceinline__ float fp8_store<float>(float v) { return v; }
+template <> __device__ __forceinline__ __nv_bfloat16 fp8_store<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+template <> __device__ __forceinline__ __half fp8_store<__half>(float v) { return __float2half_rn(v); }
+
+__device__ __forceinline__ float fp8_decode(unsigned char c) { return __half2float(__half(__nv_cvt_fp8_to_halfraw(c, __NV_E4M3))); }
+
+/* ReLU that lets NaN pass (a comparison with NaN is false) */
+__device__ __forceinline__ float fp8_act(float v, int act) { return act && v < 0.0f ? 0.0f : v; }
+
+/* ------------------------------------------------------------------ activations
+ * A half warp owns a block of 128 values of one row: 8 per lane.  q: [block][n rows][128], sx: [block][n rows]. */
+template <typename T>
+__global__ void __launch_bounds__(256) k_fp8_quantize_rows(const T *__restrict__ in, size_t ldi, unsigned char *__restrict__ q, float *__restrict__ sx,
+                                                           int n, int Nin, int kb, int vec)
+{
+    drk_dep_wait();
+    drk_dep_trigger();
+    const int sub = threadIdx.x & 15;
+    const size_t total = (size_t)n * kb, step = (size_t)gridDim.x * (blockDim.x / 16);
+    /* whole warps stay in the loop: both halves shuffle together */
+    for (size_t w0 = (size_t)blockIdx.x * (blockDim.x / 16) + (threadIdx.x >> 5) * 2; w0 < total; w0 += step) {
+        const size_t i = w0 + ((threadIdx.x >> 4) & 1);
+        const bool ok = i < total;
+        const size_t r = ok ? i / kb : 0;
+        const int b = ok ? (int)(i - r * kb) : 0, k0 = b * FP8_BLOCK + sub * 8;
+        const T *src = in + r * ldi + k0;
+        float v[8];
+        if (ok && vec && k0 + 8 <= Nin) {
+            uint4 raw[sizeof(T) / 2];
+#pragma unroll
+            for (int j = 0; j < (int)(sizeof(T) / 2); j++) raw[j] = __ldg(reinterpret_cast<const uint4 *>(src) + j);
+#pragma unroll
+            for (int j = 0; j < 8; j++) v[j] = fp8_load(reinterpret_cast<const T *>(raw) + j);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; j++) v[j] = ok && k0 + j < Nin ? fp8_load(src + j) : 0.0f;
+        }
+        float a = FP8_FLOOR;
+#pragma unroll
+        for (int j = 0; j < 8; j++) a = fmaxf(a, fabsf(v[j]));
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o));
+        const float inv = __fdiv_rn(FP8_MAX, a);
+        uint32_t c[2];
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+            const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(v[4 * j] * inv, v[4 * j + 1] * inv), __NV_SATFINITE, __NV_E4M3);
+            const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(v[4 * j + 2] * inv, v[4 * j + 3] * inv), __NV_SATFINITE, __NV_E4M3);
+            c[j] = lo | (hi << 16);
+        }
+        if (ok) {
+            *reinterpret_cast<uint2 *>(q + ((size_t)b * n + r) * FP8_BLOCK + sub * 8) = make_uint2(c[0], c[1]);
+            if (sub == 0) sx[(size_t)b * n + r] = __fdiv_rn(a, FP8_MAX);
+        }
+    }
+}
+
+/* ------------------------------------------------------------------ weights
+ * One CTA per 128 x 128 block of w [Nin][Nout]: the block goes through shared memory, once for its largest magnitude and
+ * once transposed into codes. */
+__global__ void __launch_bounds__(256) k_fp8_pack_weights(const float *__restrict__ w, unsigned char *__restrict__ codes, float *__restrict__ scales,
+                                                          int Nin, int Nout, int kb)
+{
+    __shared__ float tile[32][FP8_BLOCK + 1];
+    __shared__ float red[8];
+    const int b = blockIdx.x % kb, ob = blockIdx.x / kb;
+    float a = FP8_FLOOR;
+    for (int i = threadIdx.x; i < FP8_BLOCK_BYTES; i += 256) {
+        const int k = b * FP8_BLOCK + i / FP8_BLOCK, o = ob * FP8_BLOCK + i % FP8_BLOCK;
+        if (k < Nin && o < Nout) a = fmaxf(a, fabsf(w[(size_t)k * Nout + o]));
+    }
+    for (int s = 16; s > 0; s >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, s));
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = a;
+    __syncthreads();
+    for (int s = 0; s < 8; s++) a = fmaxf(a, red[s]);
+    const float inv = __fdiv_rn(FP8_MAX, a);
+    for (int k0 = 0; k0 < FP8_BLOCK; k0 += 32) {
+        __syncthreads();
+        for (int i = threadIdx.x; i < 32 * FP8_BLOCK; i += 256) {
+            const int k = b * FP8_BLOCK + k0 + i / FP8_BLOCK, o = ob * FP8_BLOCK + i % FP8_BLOCK;
+            tile[i / FP8_BLOCK][i % FP8_BLOCK] = k < Nin && o < Nout ? w[(size_t)k * Nout + o] * inv : 0.0f;
+        }
+        __syncthreads();
+        for (int i = threadIdx.x; i < 32 * FP8_BLOCK / 4; i += 256) {
+            const int o = i / 8, k = (i % 8) * 4;
+            const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(tile[k][o], tile[k + 1][o]), __NV_SATFINITE, __NV_E4M3);
+            const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(tile[k + 2][o], tile[k + 3][o]), __NV_SATFINITE, __NV_E4M3);
+            *reinterpret_cast<uint32_t *>(codes + (size_t)blockIdx.x * FP8_BLOCK_BYTES + o * FP8_BLOCK + k0 + k) = lo | (hi << 16);
+        }
+    }
+    if (threadIdx.x == 0) scales[blockIdx.x] = __fdiv_rn(a, FP8_MAX);
+}
+
+__global__ void __launch_bounds__(256) k_fp8_pack_codes(const unsigned char *__restrict__ src, size_t ldw, const float *__restrict__ src_scales,
+                                                        unsigned char *__restrict__ codes, float *__restrict__ scales, int Nin, int Nout, int kb)
+{
+    const int b = blockIdx.x % kb, ob = blockIdx.x / kb;
+    for (int i = threadIdx.x; i < FP8_BLOCK_BYTES; i += 256) {
+        const int o = ob * FP8_BLOCK + i / FP8_BLOCK, k = b * FP8_BLOCK + i % FP8_BLOCK;
+        codes[(size_t)blockIdx.x * FP8_BLOCK_BYTES + i] = o < Nout && k < Nin ? src[(size_t)o * ldw + k] : 0;
+    }
+    if (threadIdx.x == 0) scales[blockIdx.x] = src_scales[blockIdx.x];
+}
+
+__global__ void __launch_bounds__(256) k_fp8_unpack_weights(const unsigned char *__restrict__ codes, const float *__restrict__ scales, float *__restrict__ w,
+                                                            int Nin, int Nout, int kb)
+{
+    const int b = blockIdx.x % kb, ob = blockIdx.x / kb;
+    const float s = scales[blockIdx.x];
+    for (int i = threadIdx.x; i < FP8_BLOCK_BYTES; i += 256) {
+        const int k = b * FP8_BLOCK + i / FP8_BLOCK, o = ob * FP8_BLOCK + i % FP8_BLOCK;
+        if (k < Nin && o < Nout)
+            w[(size_t)k * Nout + o] = fp8_decode(codes[(size_t)blockIdx.x * FP8_BLOCK_BYTES + (size_t)(i % FP8_BLOCK) * FP8_BLOCK + i / FP8_BLOCK]) * s;
+    }
+}
+
+/* ------------------------------------------------------------------ product
+ * 64 rows x 64 outputs per CTA, 4 x 4 per thread; the partial sums of a block are scaled and added to the running ones. */
+template <typename T>
+__global__ void __launch_bounds__(256) k_fp8_fc(const unsigned char *__restrict__ q, const float *__restrict__ sx, const unsigned char *__restrict__ codes,
+                                                const float *__restrict__ scales, const float *__restrict__ bias, T *__restrict__ out, size_t ldo,
+                                                int n, int Nout, int kb, int otiles, int act)
+{
+    __shared__ float xs[32][65], ws[32][65];
+    drk_dep_wait();
+    drk_dep_trigger();
+    const int o0 = (blockIdx.x % otiles) * 64, tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+    const size_t r0 = (size_t)(blockIdx.x / otiles) * 64;
+    const int ob = o0 / FP8_BLOCK, orow = o0 % FP8_BLOCK;
+    float acc[4][4] = {};
+    for (int b = 0; b < kb; b++) {
+        float part[4][4] = {};
+        for (int k0 = 0; k0 < FP8_BLOCK; k0 += 32) {
+            __syncthreads();
+            for (int i = threadIdx.x; i < 64 * 32; i += 256) {
+                const int row = i / 32, k = i % 32;
+                xs[k][row] = r0 + row < (size_t)n ? fp8_decode(q[((size_t)b * n + r0 + row) * FP8_BLOCK + k0 + k]) : 0.0f;
+                ws[k][row] = fp8_decode(codes[((size_t)ob * kb + b) * FP8_BLOCK_BYTES + (size_t)(orow + row) * FP8_BLOCK + k0 + k]);
+            }
+            __syncthreads();
+            for (int k = 0; k < 32; k++)
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++) part[i][j] = fmaf(xs[k][ty + 16 * i], ws[k][tx + 16 * j], part[i][j]);
+        }
+        const float s = scales[(size_t)ob * kb + b];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float f = r0 + ty + 16 * i < (size_t)n ? sx[(size_t)b * n + r0 + ty + 16 * i] * s : 0.0f;
+#pragma unroll
+            for (int j = 0; j < 4; j++) acc[i][j] = fmaf(f, part[i][j], acc[i][j]);
+        }
+    }
+    for (int i = 0; i < 4; i++)
+        for (int j = 0; j < 4; j++) {
+            const size_t r = r0 + ty + 16 * i;
+            const int o = o0 + tx + 16 * j;
+            if (r < (size_t)n && o < Nout) out[r * ldo + o] = fp8_store<T>(fp8_act(acc[i][j] + (bias ? bias[o] : 0.0f), act));
+        }
+}
+
+/* ------------------------------------------------------------------ host side */
+struct dRk_Fp8FcPlan {
+    const void *in;
+    void *out;
+    size_t ldi, ldo;
+    int in_type, out_type, n, Nin, Nout, kb, act, dev, vec;
+    unsigned char *q;
+    float *sx;
+    const unsigned char *codes;
+    const float *scales, *bias;
+    int *status;
+};
+
+static int fp8_type_size(int type) { return type == DRK_F32 ? 4 : type == DRK_BF16 || type == DRK_F16 ? 2 : 0; }
+
+static int fp8_refuse(const char *who, const char *why)
+{
+    fprintf(stderr, "%s: %s\n", who, why);
+    return -1;
+}
+
+/* block numbers are grid indices and rows of a tensor map: both fit 31 bits */
+extern "C" int dRk_fp8_fc_supported(int n, int Nin, int Nout)
+{
+    if (n < 1 || Nin < 1 || Nout < 1) return 0;
+    const size_t wb = (size_t)fp8_blocks(Nin) * fp8_blocks(Nout), xr = (size_t)fp8_blocks(Nin) * n;
+    return wb * FP8_BLOCK < (1ull << 31) && xr < (1ull << 31) && (size_t)fp8_blocks(n) * 2 * fp8_blocks(Nout) * 2 < (1ull << 31);
+}
+
+extern "C" size_t dRk_fp8_fc_packed_bytes(int Nin, int Nout)
+{
+    if (!dRk_fp8_fc_supported(1, Nin, Nout)) return 0;
+    return (size_t)fp8_blocks(Nin) * fp8_blocks(Nout) * (FP8_BLOCK_BYTES + sizeof(float));
+}
+
+extern "C" size_t dRk_fp8_fc_scratch_bytes(int n, int Nin, int Nout)
+{
+    if (!dRk_fp8_fc_supported(n, Nin, Nout)) return 0;
+    return (size_t)fp8_blocks(Nin) * n * (FP8_BLOCK + sizeof(float));
+}
+
+static int fp8_pack_checks(const char *who, const void *src, const void *packed, int Nin, int Nout)
+{
+    if (!src || !packed) return fp8_refuse(who, "null pointer");
+    if (!dRk_fp8_fc_supported(1, Nin, Nout)) return fp8_refuse(who, "sizes outside the supported range");
+    if ((uintptr_t)packed % 16) return fp8_refuse(who, "the packed weights must start on a 16-byte boundary");
+    return 0;
+}
+
+extern "C" int dRk_fp8_fc_pack_weights(dRk_stream stream, const float *w, void *packed, int Nin, int Nout)
+{
+    const char *who = "dRk_fp8_fc_pack_weights";
+    if (fp8_pack_checks(who, w, packed, Nin, Nout)) return -1;
+    const int dev = drk_stream_device(who, stream, -1);
+    if (dev < 0) return dev;
+    const int kb = fp8_blocks(Nin), blocks = kb * fp8_blocks(Nout);
+    unsigned char *codes = (unsigned char *)packed;
+    k_fp8_pack_weights<<<blocks, 256, 0, drk_stream(stream)>>>(w, codes, (float *)(codes + (size_t)blocks * FP8_BLOCK_BYTES), Nin, Nout, kb);
+    return drk_launched(cudaGetLastError());
+}
+
+extern "C" int dRk_fp8_fc_pack_codes(dRk_stream stream, const unsigned char *src, long long ldw, const float *scales, void *packed, int Nin, int Nout)
+{
+    const char *who = "dRk_fp8_fc_pack_codes";
+    if (fp8_pack_checks(who, src, packed, Nin, Nout)) return -1;
+    if (!scales) return fp8_refuse(who, "null pointer");
+    if (ldw < Nin) return fp8_refuse(who, "rows of codes overlap (ldw < Nin)");
+    const int dev = drk_stream_device(who, stream, -1);
+    if (dev < 0) return dev;
+    const int kb = fp8_blocks(Nin), blocks = kb * fp8_blocks(Nout);
+    unsigned char *codes = (unsigned char *)packed;
+    k_fp8_pack_codes<<<blocks, 256, 0, drk_stream(stream)>>>(src, (size_t)ldw, scales, codes, (float *)(codes + (size_t)blocks * FP8_BLOCK_BYTES), Nin, Nout, kb);
+    return drk_launched(cudaGetLastError());
+}
+
+extern "C" int dRk_fp8_fc_unpack_weights(dRk_stream stream, const void *packed, float *w, int Nin, int Nout)
+{
+    const char *who = "dRk_fp8_fc_unpack_weights";
+    if (fp8_pack_checks(who, w, packed, Nin, Nout)) return -1;
+    const int dev = drk_stream_device(who, stream, -1);
+    if (dev < 0) return dev;
+    const int kb = fp8_blocks(Nin), blocks = kb * fp8_blocks(Nout);
+    const unsigned char *codes = (const unsigned char *)packed;
+    k_fp8_unpack_weights<<<blocks, 256, 0, drk_stream(stream)>>>(codes, (const float *)(codes + (size_t)blocks * FP8_BLOCK_BYTES), w, Nin, Nout, kb);
+    return drk_launched(cudaGetLastError());
+}
+
+extern "C" dRk_Fp8FcPlan *dRk_fp8_fc_plan(const void *in, int in_type, long long ldi, const void *packed, const float *bias, void *out, int out_type,
+                                          long long ldo, void *scratch, int n, int Nin, int Nout, int act, int *status)
+{
+    const char *who = "dRk_fp8_fc_plan";
+    const int isz = fp8_type_size(in_type), osz = fp8_type_size(out_type);
+    if (!in || !packed || !out || !scratch) { fp8_refuse(who, "null pointer"); return NULL; }
+    if (!isz || !osz) { fp8_refuse(who, "unknown element type"); return NULL; }
+    if (!dRk_fp8_fc_supported(n, Nin, Nout)) { fp8_refuse(who, "sizes outside the supported range"); return NULL; }
+    if (n > 1 && (ldi < Nin || ldo < Nout)) { fp8_refuse(who, "rows overlap (ldi < Nin or ldo < Nout)"); return NULL; }
+    if (ldi < 0 || ldo < 0) { fp8_refuse(who, "negative row pitch"); return NULL; }
+    if (act != 0 && act != 1) { fp8_refuse(who, "activation must be 0 (linear) or 1 (ReLU)"); return NULL; }
+    if ((uintptr_t)in % isz || (uintptr_t)out % osz || (uintptr_t)bias % 4) { fp8_refuse(who, "pointer not aligned to its element type"); return NULL; }
+    if ((uintptr_t)packed % 16 || (uintptr_t)scratch % 16) { fp8_refuse(who, "packed weights and scratch must start on a 16-byte boundary"); return NULL; }
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) { (void)cudaGetLastError(); fp8_refuse(who, "no CUDA device"); return NULL; }
+    dRk_Fp8FcPlan *p = (dRk_Fp8FcPlan *)calloc(1, sizeof(*p));
+    if (!p) { fp8_refuse(who, "out of host memory"); return NULL; }
+    p->in = in; p->out = out; p->ldi = (size_t)ldi; p->ldo = (size_t)ldo;
+    p->in_type = in_type; p->out_type = out_type;
+    p->n = n; p->Nin = Nin; p->Nout = Nout; p->kb = fp8_blocks(Nin); p->act = act; p->dev = dev;
+    p->vec = (uintptr_t)in % 16 == 0 && (n == 1 || (size_t)ldi * isz % 16 == 0);
+    p->q = (unsigned char *)scratch;
+    p->sx = (float *)(p->q + (size_t)p->kb * n * FP8_BLOCK);
+    p->codes = (const unsigned char *)packed;
+    p->scales = (const float *)(p->codes + (size_t)p->kb * fp8_blocks(Nout) * FP8_BLOCK_BYTES);
+    p->bias = bias;
+    p->status = status;
+    return p;
+}
+
+template <typename T> static int fp8_quantize(const dRk_Fp8FcPlan *p, cudaStream_t st)
+{
+    const unsigned blocks = drk_blocks((size_t)p->n * p->kb, 16, 148u * 8u);
+    return drk_launched(drk_launch_dep(k_fp8_quantize_rows<T>, dim3(blocks), dim3(256), 0, st, (const T *)p->in, p->ldi, p->q, p->sx, p->n, p->Nin, p->kb, p->vec));
+}
+
+template <typename T> static int fp8_product(const dRk_Fp8FcPlan *p, cudaStream_t st)
+{
+    const int otiles = (p->Nout + 63) / 64;
+    return drk_launched(drk_launch_dep(k_fp8_fc<T>, dim3((unsigned)otiles * ((p->n + 63) / 64)), dim3(256), 0, st, p->q, p->sx, p->codes, p->scales, p->bias,
+                                       (T *)p->out, p->ldo, p->n, p->Nout, p->kb, otiles, p->act));
+}
+
+extern "C" int dRk_fp8_fc_run(dRk_stream stream, dRk_Fp8FcPlan *p)
+{
+    if (!p) return fp8_refuse("dRk_fp8_fc_run", "no plan");
+    const int dev = drk_stream_device("dRk_fp8_fc_run", stream, p->dev);
+    if (dev < 0) return dev;
+    cudaStream_t st = drk_stream(stream);
+    const int rc = p->in_type == DRK_F32 ? fp8_quantize<float>(p, st) : p->in_type == DRK_BF16 ? fp8_quantize<__nv_bfloat16>(p, st) : fp8_quantize<__half>(p, st);
+    if (rc) return rc;
+    return p->out_type == DRK_F32 ? fp8_product<float>(p, st) : p->out_type == DRK_BF16 ? fp8_product<__nv_bfloat16>(p, st) : fp8_product<__half>(p, st);
+}
+
+extern "C" void dRk_fp8_fc_free(dRk_Fp8FcPlan *p) { free(p); }

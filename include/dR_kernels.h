@@ -231,6 +231,54 @@ dRk_TensorFcPlan *dRk_tensor_fc_x3_plan(const float *in, const float *wpacked2, 
 int dRk_tensor_fc_run(dRk_stream stream, dRk_TensorFcPlan *plan);
 void dRk_tensor_fc_free(dRk_TensorFcPlan *plan);
 
+/* Element types of the operators below; the graph nodes use DRK_F32. */
+enum { DRK_F32 = 0, DRK_BF16 = 1, DRK_F16 = 2 };
+
+/*
+ * Fully connected layer with its operands in 8-bit floating point (e4m3) and a float scale for each block of 128:
+ *   out[r][o] = act(bias[o] + sum_b sx[r][b] sw[o/128][b] sum_{k in block b} qx[r][k] qw[o][k])
+ * The weights are stored that way (a quarter of the bytes of dRk_fc_f32, one scale per 128 x 128 block), the input is
+ * rounded when the layer runs: with A = max(largest |x| of a row's block of 128, 2^-96) in 32 bits, qx = e4m3(x * (448 / A)),
+ * to nearest even, and sx = A / 448.  Sums are held in 32 bits on the way.  No counterpart in the reference, which is FP32
+ * only (Kernels/dR_fcl.cl:59-120); an output's error against dRk_fc_f32 is that of operands with 4 significant bits.
+ *   in  : n rows of Nin values of in_type, ldi elements apart;  out : n rows of Nout values of out_type, ldo elements apart
+ *         (what lies between Nout and ldo is left as it is);  bias : Nout floats or NULL;  act : 0 linear, 1 ReLU (NaN passes)
+ *   packed : dRk_fp8_fc_packed_bytes() bytes, scratch : dRk_fp8_fc_scratch_bytes() bytes, both on 16-byte boundaries.
+ * A row that holds an infinity or a NaN becomes NaN; the other rows do not see it.
+ * A plan keeps the pointers it was made with and belongs to the device that was current; run refuses another one, or another
+ * device's stream (-6).  Runs of plans that share a scratch or an output must not overlap on the GPU; neither must two runs of
+ * one plan on two streams.  A run only enqueues (two launches), allocates nothing and may be captured into a CUDA graph.
+ * `status` (may be NULL) as dRk_tensor_conv_plan.  _plan returns NULL, the others a negative value, with a message on stderr,
+ * for arguments that they refuse.
+ */
+typedef struct dRk_Fp8FcPlan dRk_Fp8FcPlan;
+int dRk_fp8_fc_supported(int n, int Nin, int Nout);
+size_t dRk_fp8_fc_packed_bytes(int Nin, int Nout);
+size_t dRk_fp8_fc_scratch_bytes(int n, int Nin, int Nout);
+/* from the reference's [Nin][Nout] matrix, on the device: scale = max(largest |w| of the block, 2^-96) / 448 */
+int dRk_fp8_fc_pack_weights(dRk_stream stream, const float *w, void *packed, int Nin, int Nout);
+/* from weights that are e4m3 already: codes [Nout][Nin] with rows ldw bytes apart, scales [ceil(Nout/128)][ceil(Nin/128)] */
+int dRk_fp8_fc_pack_codes(dRk_stream stream, const unsigned char *codes, long long ldw, const float *scales, void *packed, int Nin, int Nout);
+/* the [Nin][Nout] matrix that packed weights stand for */
+int dRk_fp8_fc_unpack_weights(dRk_stream stream, const void *packed, float *w, int Nin, int Nout);
+dRk_Fp8FcPlan *dRk_fp8_fc_plan(const void *in, int in_type, long long ldi, const void *packed, const float *bias, void *out, int out_type,
+                               long long ldo, void *scratch, int n, int Nin, int Nout, int act, int *status);
+int dRk_fp8_fc_run(dRk_stream stream, dRk_Fp8FcPlan *plan);
+void dRk_fp8_fc_free(dRk_Fp8FcPlan *plan);
+
+/*
+ * Scores of n rows of `len` logits v (ld elements apart) at a temperature 1 / scale, in one pass over them:
+ *   logprob [n][m]      scale * v[label] - log sum exp(scale * v) for the m labels of each row (labels [n][m]);
+ *                       0 for a negative label ("none given"), NaN for one that is not below len
+ *   entropy [n]         -sum p log p (natural logarithm); NULL: not wanted
+ *   top_logprob, top_index [n][k]  the k <= min(32, len) largest logits, descending, equal ones by ascending index, NaN first
+ * Logits of -inf have probability 0 (a mask); a row of nothing else scores -inf everywhere, its entropy is 0.  A NaN or +inf
+ * makes every score of its row NaN (the order of the alternatives stands).  m = 0 and k = 0 are allowed.  Sums are held in 32 bits.  Next to dRk_softmax (src/dR_nodes_math.c:620-678), which writes the probabilities themselves.
+ * One launch, no workspace; -1 (with a message on stderr) for refused arguments, -6 for another device's stream.
+ */
+int dRk_logprobs(dRk_stream stream, const void *logits, int type, long long ld, int n, int len, float scale, const int *labels, int m,
+                 float *logprob, float *entropy, int k, float *top_logprob, int *top_index);
+
 /* Test support for the bounded waits of the tensor-core kernels (no counterpart in the reference, whose failure path is
  * the return code of its OpenCL calls, src/dR_clwrap.c:874-883): one CTA waits at most `limit_cycles` SM clocks on a
  * barrier nothing arrives at, through the kernels' own wait function; it then writes code 9 to `status`, as a kernel
