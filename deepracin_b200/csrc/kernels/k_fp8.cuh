@@ -1,0 +1,38 @@
+/* What the translation units of the 8-bit fully connected layer share: sizes, element types, and the launchers of its products. */
+#pragma once
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+#include "k_common.cuh"
+
+#define FP8_BLOCK 128                                   /* values under one scale, rows of a packed block, bytes of its rows */
+#define FP8_BLOCK_BYTES (FP8_BLOCK * FP8_BLOCK)
+
+static inline int fp8_blocks(int n) { return (int)(((long long)n + FP8_BLOCK - 1) / FP8_BLOCK); }
+
+template <typename T> __device__ __forceinline__ T fp8_store(float v);
+template <> __device__ __forceinline__ float fp8_store<float>(float v) { return v; }
+template <> __device__ __forceinline__ __nv_bfloat16 fp8_store<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+template <> __device__ __forceinline__ __half fp8_store<__half>(float v) { return __float2half_rn(v); }
+
+/* ReLU that lets NaN pass (a comparison with NaN is false) */
+__device__ __forceinline__ float fp8_act(float v, int act) { return act && v < 0.0f ? 0.0f : v; }
+
+struct Fp8Params {
+    const float *sx, *scales, *bias;    /* sx [kb][n], scales [ob][kb] */
+    void *out;
+    size_t ldo;
+    int out_type, n, Nout, kb, ob, act;
+    int *status;
+};
+
+/* which product a layer's shape runs on, and its tensor maps */
+struct Fp8Tensor {
+    CUtensorMap mapW, mapX;
+    int nt;                             /* rows per tile of k_fp8_swap */
+    int split;                          /* CTAs of a cluster that share a tile's K blocks */
+};
+
+int drk_fp8_tensor_plan(Fp8Tensor *t, const Fp8Params *p, const void *codes, const void *q, int sms);
+int drk_fp8_tensor_launch(cudaStream_t st, const Fp8Tensor *t, const Fp8Params *p);

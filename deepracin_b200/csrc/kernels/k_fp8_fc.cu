@@ -12,31 +12,17 @@
  */
 #include <math.h>
 #include <stdio.h>
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
-#include <cuda_fp8.h>
-#include "k_common.cuh"
+#include <stdlib.h>
+#include "k_fp8.cuh"
 
-#define FP8_BLOCK 128
-#define FP8_BLOCK_BYTES (FP8_BLOCK * FP8_BLOCK)
 #define FP8_MAX 448.0f
 #define FP8_FLOOR 0x1p-96f      /* smallest block maximum a scale is made from: 448 / A stays finite */
-
-static int fp8_blocks(int n) { return (int)(((long long)n + FP8_BLOCK - 1) / FP8_BLOCK); }
 
 template <typename T> __device__ __forceinline__ float fp8_load(const T *p);
 template <> __device__ __forceinline__ float fp8_load(const float *p) { return *p; }
 template <> __device__ __forceinline__ float fp8_load(const __nv_bfloat16 *p) { return __bfloat162float(*p); }
 template <> __device__ __forceinline__ float fp8_load(const __half *p) { return __half2float(*p); }
-template <typename T> __device__ __forceinline__ T fp8_store(float v);
-template <> __device__ __forceinline__ float fp8_store<float>(float v) { return v; }
-template <> __device__ __forceinline__ __nv_bfloat16 fp8_store<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
-template <> __device__ __forceinline__ __half fp8_store<__half>(float v) { return __float2half_rn(v); }
-
 __device__ __forceinline__ float fp8_decode(unsigned char c) { return __half2float(__half(__nv_cvt_fp8_to_halfraw(c, __NV_E4M3))); }
-
-/* ReLU that lets NaN pass (a comparison with NaN is false) */
-__device__ __forceinline__ float fp8_act(float v, int act) { return act && v < 0.0f ? 0.0f : v; }
 
 /* ------------------------------------------------------------------ activations
  * A half warp owns a block of 128 values of one row: 8 per lane.  q: [block][n rows][128], sx: [block][n rows]. */
@@ -145,63 +131,15 @@ __global__ void __launch_bounds__(256) k_fp8_unpack_weights(const unsigned char 
     }
 }
 
-/* ------------------------------------------------------------------ product
- * 64 rows x 64 outputs per CTA, 4 x 4 per thread; the partial sums of a block are scaled and added to the running ones. */
-template <typename T>
-__global__ void __launch_bounds__(256) k_fp8_fc(const unsigned char *__restrict__ q, const float *__restrict__ sx, const unsigned char *__restrict__ codes,
-                                                const float *__restrict__ scales, const float *__restrict__ bias, T *__restrict__ out, size_t ldo,
-                                                int n, int Nout, int kb, int otiles, int act)
-{
-    __shared__ float xs[32][65], ws[32][65];
-    drk_dep_wait();
-    drk_dep_trigger();
-    const int o0 = (blockIdx.x % otiles) * 64, tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-    const size_t r0 = (size_t)(blockIdx.x / otiles) * 64;
-    const int ob = o0 / FP8_BLOCK, orow = o0 % FP8_BLOCK;
-    float acc[4][4] = {};
-    for (int b = 0; b < kb; b++) {
-        float part[4][4] = {};
-        for (int k0 = 0; k0 < FP8_BLOCK; k0 += 32) {
-            __syncthreads();
-            for (int i = threadIdx.x; i < 64 * 32; i += 256) {
-                const int row = i / 32, k = i % 32;
-                xs[k][row] = r0 + row < (size_t)n ? fp8_decode(q[((size_t)b * n + r0 + row) * FP8_BLOCK + k0 + k]) : 0.0f;
-                ws[k][row] = fp8_decode(codes[((size_t)ob * kb + b) * FP8_BLOCK_BYTES + (size_t)(orow + row) * FP8_BLOCK + k0 + k]);
-            }
-            __syncthreads();
-            for (int k = 0; k < 32; k++)
-#pragma unroll
-                for (int i = 0; i < 4; i++)
-#pragma unroll
-                    for (int j = 0; j < 4; j++) part[i][j] = fmaf(xs[k][ty + 16 * i], ws[k][tx + 16 * j], part[i][j]);
-        }
-        const float s = scales[(size_t)ob * kb + b];
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const float f = r0 + ty + 16 * i < (size_t)n ? sx[(size_t)b * n + r0 + ty + 16 * i] * s : 0.0f;
-#pragma unroll
-            for (int j = 0; j < 4; j++) acc[i][j] = fmaf(f, part[i][j], acc[i][j]);
-        }
-    }
-    for (int i = 0; i < 4; i++)
-        for (int j = 0; j < 4; j++) {
-            const size_t r = r0 + ty + 16 * i;
-            const int o = o0 + tx + 16 * j;
-            if (r < (size_t)n && o < Nout) out[r * ldo + o] = fp8_store<T>(fp8_act(acc[i][j] + (bias ? bias[o] : 0.0f), act));
-        }
-}
-
 /* ------------------------------------------------------------------ host side */
 struct dRk_Fp8FcPlan {
     const void *in;
-    void *out;
-    size_t ldi, ldo;
-    int in_type, out_type, n, Nin, Nout, kb, act, dev, vec;
+    size_t ldi;
+    int in_type, Nin, dev, vec;
     unsigned char *q;
     float *sx;
-    const unsigned char *codes;
-    const float *scales, *bias;
-    int *status;
+    Fp8Params p;
+    Fp8Tensor t;
 };
 
 static int fp8_type_size(int type) { return type == DRK_F32 ? 4 : type == DRK_BF16 || type == DRK_F16 ? 2 : 0; }
@@ -295,30 +233,38 @@ extern "C" dRk_Fp8FcPlan *dRk_fp8_fc_plan(const void *in, int in_type, long long
     if (cudaGetDevice(&dev) != cudaSuccess) { (void)cudaGetLastError(); fp8_refuse(who, "no CUDA device"); return NULL; }
     dRk_Fp8FcPlan *p = (dRk_Fp8FcPlan *)calloc(1, sizeof(*p));
     if (!p) { fp8_refuse(who, "out of host memory"); return NULL; }
-    p->in = in; p->out = out; p->ldi = (size_t)ldi; p->ldo = (size_t)ldo;
-    p->in_type = in_type; p->out_type = out_type;
-    p->n = n; p->Nin = Nin; p->Nout = Nout; p->kb = fp8_blocks(Nin); p->act = act; p->dev = dev;
+    p->in = in;
+    p->ldi = (size_t)ldi;
+    p->in_type = in_type;
+    p->Nin = Nin;
+    p->dev = dev;
     p->vec = (uintptr_t)in % 16 == 0 && (n == 1 || (size_t)ldi * isz % 16 == 0);
+    const int kb = fp8_blocks(Nin), ob = fp8_blocks(Nout);
+    const unsigned char *codes = (const unsigned char *)packed;
     p->q = (unsigned char *)scratch;
-    p->sx = (float *)(p->q + (size_t)p->kb * n * FP8_BLOCK);
-    p->codes = (const unsigned char *)packed;
-    p->scales = (const float *)(p->codes + (size_t)p->kb * fp8_blocks(Nout) * FP8_BLOCK_BYTES);
-    p->bias = bias;
-    p->status = status;
+    p->sx = (float *)(p->q + (size_t)kb * n * FP8_BLOCK);
+    p->p.sx = p->sx;
+    p->p.scales = (const float *)(codes + (size_t)kb * ob * FP8_BLOCK_BYTES);
+    p->p.bias = bias;
+    p->p.out = out;
+    p->p.ldo = (size_t)ldo;
+    p->p.out_type = out_type;
+    p->p.n = n; p->p.Nout = Nout; p->p.kb = kb; p->p.ob = ob; p->p.act = act;
+    p->p.status = status;
+    int sms = 148;
+    if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || drk_fp8_tensor_plan(&p->t, &p->p, codes, p->q, sms)) {
+        (void)cudaGetLastError();
+        fp8_refuse(who, "tensor maps could not be made");
+        free(p);
+        return NULL;
+    }
     return p;
 }
 
 template <typename T> static int fp8_quantize(const dRk_Fp8FcPlan *p, cudaStream_t st)
 {
-    const unsigned blocks = drk_blocks((size_t)p->n * p->kb, 16, 148u * 8u);
-    return drk_launched(drk_launch_dep(k_fp8_quantize_rows<T>, dim3(blocks), dim3(256), 0, st, (const T *)p->in, p->ldi, p->q, p->sx, p->n, p->Nin, p->kb, p->vec));
-}
-
-template <typename T> static int fp8_product(const dRk_Fp8FcPlan *p, cudaStream_t st)
-{
-    const int otiles = (p->Nout + 63) / 64;
-    return drk_launched(drk_launch_dep(k_fp8_fc<T>, dim3((unsigned)otiles * ((p->n + 63) / 64)), dim3(256), 0, st, p->q, p->sx, p->codes, p->scales, p->bias,
-                                       (T *)p->out, p->ldo, p->n, p->Nout, p->kb, otiles, p->act));
+    const unsigned blocks = drk_blocks((size_t)p->p.n * p->p.kb, 16, 148u * 8u);
+    return drk_launched(drk_launch_dep(k_fp8_quantize_rows<T>, dim3(blocks), dim3(256), 0, st, (const T *)p->in, p->ldi, p->q, p->sx, p->p.n, p->Nin, p->p.kb, p->vec));
 }
 
 extern "C" int dRk_fp8_fc_run(dRk_stream stream, dRk_Fp8FcPlan *p)
@@ -329,7 +275,7 @@ extern "C" int dRk_fp8_fc_run(dRk_stream stream, dRk_Fp8FcPlan *p)
     cudaStream_t st = drk_stream(stream);
     const int rc = p->in_type == DRK_F32 ? fp8_quantize<float>(p, st) : p->in_type == DRK_BF16 ? fp8_quantize<__nv_bfloat16>(p, st) : fp8_quantize<__half>(p, st);
     if (rc) return rc;
-    return p->out_type == DRK_F32 ? fp8_product<float>(p, st) : p->out_type == DRK_BF16 ? fp8_product<__nv_bfloat16>(p, st) : fp8_product<__half>(p, st);
+    return drk_fp8_tensor_launch(st, &p->t, &p->p);
 }
 
 extern "C" void dRk_fp8_fc_free(dRk_Fp8FcPlan *p) { free(p); }
