@@ -20,16 +20,17 @@ template <> __device__ __forceinline__ __half fp8_store<__half>(float v) { retur
 __device__ __forceinline__ float fp8_act(float v, int act) { return act && v < 0.0f ? 0.0f : v; }
 
 struct Fp8Params {
-    const float *sx, *scales, *bias;    /* sx [kb][n], scales [ob][kb] */
+    const float *sx, *scales, *bias;    /* sx [n][kbp], scales [ob][kb] */
     void *out;
     size_t ldo;
-    int out_type, n, Nout, kb, ob, act;
+    int out_type, n, Nout, kb, kbp, ob, act;   /* kbp: kb rounded up to four */
     int *status;
 };
 
 /* which product a layer's shape runs on, and its tensor maps */
 struct Fp8Tensor {
     CUtensorMap mapW, mapX;
+    int pairs, mtiles, ntiles;          /* k_fp8_pair: pairs of CTAs, tiles of 256 rows and of 256 outputs; pairs = 0: k_fp8_swap */
     int nt;                             /* rows per tile of k_fp8_swap */
     int split;                          /* CTAs of a cluster that share a tile's K blocks */
 };

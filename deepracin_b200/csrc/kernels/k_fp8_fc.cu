@@ -25,10 +25,10 @@ template <> __device__ __forceinline__ float fp8_load(const __half *p) { return 
 __device__ __forceinline__ float fp8_decode(unsigned char c) { return __half2float(__half(__nv_cvt_fp8_to_halfraw(c, __NV_E4M3))); }
 
 /* ------------------------------------------------------------------ activations
- * A half warp owns a block of 128 values of one row: 8 per lane.  q: [block][n rows][128], sx: [block][n rows]. */
+ * A half warp owns a block of 128 values of one row: 8 per lane.  q: [block][n rows][128], sx: [n rows][kbp blocks]. */
 template <typename T>
 __global__ void __launch_bounds__(256) k_fp8_quantize_rows(const T *__restrict__ in, size_t ldi, unsigned char *__restrict__ q, float *__restrict__ sx,
-                                                           int n, int Nin, int kb, int vec)
+                                                           int n, int Nin, int kb, int kbp, int vec)
 {
     drk_dep_wait();
     drk_dep_trigger();
@@ -67,7 +67,7 @@ __global__ void __launch_bounds__(256) k_fp8_quantize_rows(const T *__restrict__
         }
         if (ok) {
             *reinterpret_cast<uint2 *>(q + ((size_t)b * n + r) * FP8_BLOCK + sub * 8) = make_uint2(c[0], c[1]);
-            if (sub == 0) sx[(size_t)b * n + r] = __fdiv_rn(a, FP8_MAX);
+            if (sub == 0) sx[r * kbp + b] = __fdiv_rn(a, FP8_MAX);
         }
     }
 }
@@ -167,7 +167,7 @@ extern "C" size_t dRk_fp8_fc_packed_bytes(int Nin, int Nout)
 extern "C" size_t dRk_fp8_fc_scratch_bytes(int n, int Nin, int Nout)
 {
     if (!dRk_fp8_fc_supported(n, Nin, Nout)) return 0;
-    return (size_t)fp8_blocks(Nin) * n * (FP8_BLOCK + sizeof(float));
+    return (size_t)n * (fp8_blocks(Nin) * (size_t)FP8_BLOCK + (size_t)((fp8_blocks(Nin) + 3) & ~3) * sizeof(float));
 }
 
 static int fp8_pack_checks(const char *who, const void *src, const void *packed, int Nin, int Nout)
@@ -249,7 +249,7 @@ extern "C" dRk_Fp8FcPlan *dRk_fp8_fc_plan(const void *in, int in_type, long long
     p->p.out = out;
     p->p.ldo = (size_t)ldo;
     p->p.out_type = out_type;
-    p->p.n = n; p->p.Nout = Nout; p->p.kb = kb; p->p.ob = ob; p->p.act = act;
+    p->p.n = n; p->p.Nout = Nout; p->p.kb = kb; p->p.kbp = (kb + 3) & ~3; p->p.ob = ob; p->p.act = act;
     p->p.status = status;
     int sms = 148;
     if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || drk_fp8_tensor_plan(&p->t, &p->p, codes, p->q, sms)) {
@@ -264,7 +264,7 @@ extern "C" dRk_Fp8FcPlan *dRk_fp8_fc_plan(const void *in, int in_type, long long
 template <typename T> static int fp8_quantize(const dRk_Fp8FcPlan *p, cudaStream_t st)
 {
     const unsigned blocks = drk_blocks((size_t)p->p.n * p->p.kb, 16, 148u * 8u);
-    return drk_launched(drk_launch_dep(k_fp8_quantize_rows<T>, dim3(blocks), dim3(256), 0, st, (const T *)p->in, p->ldi, p->q, p->sx, p->p.n, p->Nin, p->p.kb, p->vec));
+    return drk_launched(drk_launch_dep(k_fp8_quantize_rows<T>, dim3(blocks), dim3(256), 0, st, (const T *)p->in, p->ldi, p->q, p->sx, p->p.n, p->Nin, p->p.kb, p->p.kbp, p->vec));
 }
 
 extern "C" int dRk_fp8_fc_run(dRk_stream stream, dRk_Fp8FcPlan *p)

@@ -26,10 +26,44 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16])
                  : "r"(taddr) : "memory");
     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
+/* One statement loads and waits: with a wait of its own that names the registers as its operands, the compiler copied them, and
+ * k_fp8_pair's additions took three times as long. */
+__device__ __forceinline__ void tmem_ld64(uint32_t taddr, uint32_t (&r)[64])
+{
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x64.b32 "
+                 "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+                 "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, "
+                 "%32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, "
+                 "%48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63}, [%64];\n\t"
+                 "tcgen05.wait::ld.sync.aligned;"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+                   "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+                   "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+                   "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]),
+                   "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]),
+                   "=r"(r[40]), "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]),
+                   "=r"(r[48]), "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]),
+                   "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63])
+                 : "r"(taddr) : "memory");
+}
 /* two FP32 FMAs in one instruction */
 __device__ __forceinline__ void ffma2(unsigned long long &acc, unsigned long long a, uint32_t b0, uint32_t b1)
 {
     asm("{\n\t.reg .b64 b;\n\tmov.b64 b, {%2, %3};\n\tfma.rn.f32x2 %0, %1, b, %0;\n\t}" : "+l"(acc) : "l"(a), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ bool elect_one()
+{
+    uint32_t one;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+    return one != 0;
+}
+/* whether a phase is over, without waiting for it (try_wait suspends the thread for a while) */
+__device__ __forceinline__ uint32_t mbar_test(uint32_t bar, uint32_t parity)
+{
+    uint32_t ok;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    return ok;
 }
 __device__ __forceinline__ uint32_t cluster_rank() { uint32_t r; asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
 __device__ __forceinline__ void cluster_sync()
@@ -166,25 +200,33 @@ k_fp8_swap(const __grid_constant__ CUtensorMap mapW, const __grid_constant__ CUt
         const int quarter = warp & 3;
         float *mine = factors + quarter * 2 * NT;
         constexpr int PER = (NT + 31) / 32;
-        float next[PER];
+        float4 now[PER], next[PER];     /* sx of this lane's rows for the blocks of a group of four, and for the next group */
+        float sw, sw_next;
         drk_dep_wait();     /* sx is written by the launch in front */
         auto fetch = [&](int b) {
-            const float s = __ldg(p.scales + (size_t)ot * p.kb + b);
 #pragma unroll
             for (int j = 0; j < PER; j++) {
                 const int r = j * 32 + lane;
-                next[j] = r < NT && r0 + r < p.n ? __ldg(p.sx + (size_t)b * p.n + r0 + r) * s : 0.0f;
+                next[j] = r < NT && r0 + r < p.n ? __ldcg(reinterpret_cast<const float4 *>(p.sx + (size_t)(r0 + r) * p.kbp + (b & ~3))) : make_float4(0.f, 0.f, 0.f, 0.f);
             }
         };
-        if (b0 < b1) fetch(b0);
+        const float *swp = p.scales + (size_t)ot * p.kb;
+        if (b0 < b1) { fetch(b0); sw_next = __ldg(swp + b0); }
         int slot = 0, flip = 0;
         uint32_t sphase = 0;
         for (int b = b0; b < b1; b++) {
             float *f = mine + flip * NT;
+            if (b == b0 || (b & 3) == 0) {
 #pragma unroll
-            for (int j = 0; j < PER; j++) if (j * 32 + lane < NT) f[j * 32 + lane] = next[j];
+                for (int j = 0; j < PER; j++) now[j] = next[j];
+                if ((b | 3) + 1 < b1) fetch((b | 3) + 1);
+            }
+            sw = sw_next;
+            if (b + 1 < b1) sw_next = __ldg(swp + b + 1);
+#pragma unroll
+            for (int j = 0; j < PER; j++)
+                if (j * 32 + lane < NT) f[j * 32 + lane] = ((b & 2) ? ((b & 1) ? now[j].w : now[j].z) : ((b & 1) ? now[j].y : now[j].x)) * sw;
             __syncwarp();
-            if (b + 1 < b1) fetch(b + 1);
             if (!mbar_wait_warp(tfull_bar(slot), sphase, abort_flag, p.status, 34)) break;
             tc_fence_after();
             const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(slot * NT);
@@ -242,6 +284,317 @@ k_fp8_swap(const __grid_constant__ CUtensorMap mapW, const __grid_constant__ CUt
     cluster_sync();     /* the other CTAs read this one's sums until here */
 }
 
+/* a wait of a whole warp that holds many registers: no call inside, which would have them saved around it */
+__device__ __forceinline__ bool mbar_wait_warp_inline(uint32_t bar, uint32_t parity, volatile int *abort_flag, int *status, int code)
+{
+    bool ok = mbar_try(bar, parity);
+    if (!__all_sync(0xffffffffu, ok)) {
+        const long long t0 = clock64();
+        while (!ok && !*abort_flag) {
+            ok = mbar_try(bar, parity);
+            if (!ok && clock64() - t0 > WAIT_CYCLES) {
+                *abort_flag = 1;
+                if (status) atomicExch(status, code);
+            }
+        }
+    }
+    return __all_sync(0xffffffffu, ok);
+}
+
+/* the same for one thread */
+__device__ __forceinline__ bool mbar_wait1(uint32_t bar, uint32_t parity, volatile int *abort_flag, int *status, int code)
+{
+    if (mbar_try(bar, parity)) return true;     /* reading the clock costs as much as half an MMA: not on this way */
+    const long long t0 = clock64();
+    while (!mbar_try(bar, parity)) {
+        if (*abort_flag) return false;
+        if (clock64() - t0 > WAIT_CYCLES) { *abort_flag = 1; if (status) atomicExch(status, code); return false; }
+    }
+    return true;
+}
+/*
+ * Many rows: a pair of CTAs (cta_group::2) computes 256 rows x 256 outputs, persistent over the tiles.  Per 128 inputs each CTA
+ * fetches its 128 rows of the input and 64 rows of each of the tile's two weight blocks (32 KiB a stage; a single CTA's tile of
+ * 128 x 256 would fetch 48), counted on the leader's barriers.  Two warps of the leader issue, one for each weight block (M = 256,
+ * N = 128, four MMAs of K = 32), into one of two accumulators per block; the commits tell both CTAs.  Warps 4-11 own 32 rows and
+ * one weight block each: they read the accumulator, hand its slot back, and add it times sx * sw to 128 sums per lane.
+ *
+ * What bounds it: the way issue -> commit -> read -> hand back -> issue, about 1000 clocks with two accumulators under way, where
+ * the MMAs of a block take 512.  4096 x 8192 -> 8192: 290 us with the rounding of the input (1.9 PFLOP/s); without the sums (copy
+ * and MMAs alone) 207 us.  Measured on the way there: all sums in one accumulator of 256 columns and one issuing lane 309-320 us;
+ * additions as packed FFMA2 over registers that had to be paired up 370 us and more; a cluster-scope release on the hand-back
+ * (a memory barrier) 450 us.
+ */
+struct PairCfg {
+    static constexpr int STAGE_BYTES = 2 * FP8_BLOCK_BYTES;
+    static constexpr int STAGES = 6;
+    static constexpr int STG_PITCH = 33;                        /* floats per row of a warp's 32 x 32 transposing stage */
+    static constexpr int SMEM = 1024 + STAGES * STAGE_BYTES + 8 * 32 * STG_PITCH * 4 + 256;
+    static constexpr int GROUP = 8;                             /* row tiles that are walked together before the next outputs */
+};
+
+__device__ __forceinline__ void umma_f8_pair(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate)
+{
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
+                 ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate) : "memory");
+}
+/* both CTAs' barriers at this address are arrived at once all MMAs issued so far have completed */
+__device__ __forceinline__ void umma_commit_pair(uint32_t bar)
+{
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"((uint16_t)3) : "memory");
+}
+/* a copy into this CTA's shared memory that is counted on a barrier of the pair's leader */
+__device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const CUtensorMap *map, int c0, int c1, uint32_t cluster_bar)
+{
+    asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+                 ::"r"(dst), "l"(map), "r"(c0), "r"(c1), "r"(cluster_bar) : "memory");
+}
+__device__ __forceinline__ uint32_t leader_addr(uint32_t saddr) { uint32_t a; asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(a) : "r"(saddr)); return a; }
+__device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_bar)
+{
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
+}
+
+__global__ void __launch_bounds__(384, 1)
+k_fp8_pair(const __grid_constant__ CUtensorMap mapW, const __grid_constant__ CUtensorMap mapX, const Fp8Params p, int mtiles, int ntiles)
+{
+    using C = PairCfg;
+    extern __shared__ char smem_raw[];
+    const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    char *gen = smem_raw + (base - smem_u32(smem_raw));
+    float *stage_out = reinterpret_cast<float *>(gen + C::STAGES * C::STAGE_BYTES);
+    char *tail = reinterpret_cast<char *>(stage_out + 8 * 32 * C::STG_PITCH);
+    const uint32_t bars = smem_u32(tail);
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(tail + 8 * (2 * C::STAGES + 10));
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
+    auto full_bar = [&](int s) { return bars + 8u * s; };
+    auto empty_bar = [&](int s) { return bars + 8u * (C::STAGES + s); };
+    auto tfull_bar = [&](int a) { return bars + 8u * (2 * C::STAGES + a); };
+    auto tempty_bar = [&](int a) { return bars + 8u * (2 * C::STAGES + 4 + a); };
+    const uint32_t drain_bar = bars + 8u * (2 * C::STAGES + 8);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = (int)cluster_rank();
+    const bool leader = rank == 0;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < C::STAGES; s++) { mbar_init(full_bar(s), 1); mbar_init(empty_bar(s), 2); }
+        for (int a = 0; a < 4; a++) { mbar_init(tfull_bar(a), 1); mbar_init(tempty_bar(a), 8); }
+        for (int h = 0; h < 2; h++) mbar_init(drain_bar + 8u * h, 1);
+        *abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync();     /* the partner's barriers are ready, and its TMEM */
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+
+    const int tiles = mtiles * ntiles, pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+    /* tile t -> row tile, output tile: GROUP row tiles by all output tiles at a time, so that the tiles in flight share both operands */
+    auto place = [&](int t, int &mt, int &nt) {
+        const int per = C::GROUP * ntiles, g = t / per, left = t - g * per;
+        const int rows = min(C::GROUP, mtiles - g * C::GROUP);
+        nt = left / rows;
+        mt = g * C::GROUP + left - nt * rows;
+    };
+
+    if (warp < 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        if (warp == 0) {
+            if (lane == 0) {
+                const uint32_t leader_full = leader_addr(full_bar(0));
+                int pre = 0, mt, nt;
+                /* this CTA's 64 rows of the two weight blocks of a tile: the pair's MMA over N = 128 takes half of B from each CTA */
+                auto load_w = [&](uint32_t dst, int ntile, int b, uint32_t bar) {
+                    for (int h = 0; h < 2; h++)
+                        tma_load_2d_pair(dst + h * (FP8_BLOCK_BYTES / 2), &mapW, 0,
+                                         ((2 * ntile + h) * p.kb + b) * FP8_BLOCK + rank * 64, bar);
+                };
+                if (pair < tiles) {
+                    place(pair, mt, nt);
+                    for (; pre < C::STAGES && pre < p.kb; pre++) {      /* weights first, as in k_fp8_swap */
+                        if (leader) mbar_expect_tx(full_bar(pre), 2 * C::STAGE_BYTES);
+                        load_w(base + pre * C::STAGE_BYTES + FP8_BLOCK_BYTES, nt, pre, leader_full + 8u * pre);
+                    }
+                }
+                drk_dep_wait();
+                int stage = 0;
+                uint32_t phase = 0;
+                long long issued = 0;
+                bool ok = true;
+                for (int t = pair; t < tiles && ok; t += pairs) {
+                    place(t, mt, nt);
+                    for (int b = 0; b < p.kb; b++) {
+                        const uint32_t sa = base + stage * C::STAGE_BYTES, bar = leader_full + 8u * stage;
+                        if (issued >= pre) {
+                            if (!mbar_wait1(empty_bar(stage), phase ^ 1u, abort_flag, p.status, 41)) { ok = false; break; }
+                            if (leader) mbar_expect_tx(full_bar(stage), 2 * C::STAGE_BYTES);
+                            load_w(sa + FP8_BLOCK_BYTES, nt, b, bar);
+                        }
+                        tma_load_2d_pair(sa, &mapX, 0, b * p.n + mt * 256 + rank * 128, bar);
+                        issued++;
+                        if (++stage == C::STAGES) { stage = 0; phase ^= 1u; }
+                    }
+                }
+                if (!ok && leader) {        /* no copy may land after the exit: the leader's barriers count both CTAs' */
+                    const long long pending = issued < C::STAGES ? issued : C::STAGES;
+                    for (long long i = 0; i < pending; i++) {
+                        if (--stage < 0) { stage = C::STAGES - 1; phase ^= 1u; }
+                        const long long t0 = clock64();
+                        while (!mbar_try(full_bar(stage), phase) && clock64() - t0 < WAIT_CYCLES) { }
+                    }
+                }
+            }
+        } else if (warp < 3 && leader) {
+            /* Two issuers, one for each weight block of a tile: what one spends on its two waits, the other's MMAs cover.  The whole
+               warp walks the loop and one elected lane issues, so that the descriptors live in uniform registers. */
+            constexpr uint32_t idesc = make_idesc_f8(256, 128);
+            const int h = warp - 1;
+            int stage = 0, slot = 0;
+            uint32_t phase = 0, sphase = 0;
+            bool ok = true;
+            for (int t = pair; t < tiles && ok; t += pairs)
+                for (int b = 0; b < p.kb; b++) {
+                    const bool full = mbar_try(full_bar(stage), phase), room = mbar_try(tempty_bar(2 * h + slot), sphase ^ 1u);
+                    if (!__all_sync(0xffffffffu, full && room) &&
+                        (!mbar_wait_warp_inline(full_bar(stage), phase, abort_flag, p.status, 43) ||
+                         !mbar_wait_warp_inline(tempty_bar(2 * h + slot), sphase ^ 1u, abort_flag, p.status, 42))) { ok = false; break; }
+                    tc_fence_after();
+                    if (elect_one()) {
+                        const uint32_t sa = base + stage * C::STAGE_BYTES;
+                        const uint64_t adesc = make_smem_desc(sa), bdesc = make_smem_desc(sa + FP8_BLOCK_BYTES + h * (FP8_BLOCK_BYTES / 2));
+#pragma unroll
+                        for (int j = 0; j < 4; j++)
+                            umma_f8_pair(tmem_base + (uint32_t)(slot * 256 + h * 128), adesc + (uint64_t)(j * 2), bdesc + (uint64_t)(j * 2), idesc, j ? 1u : 0u);
+                        umma_commit_pair(tfull_bar(2 * h + slot));
+                        umma_commit_pair(empty_bar(stage));
+                    }
+                    __syncwarp();
+                    if (++stage == C::STAGES) { stage = 0; phase ^= 1u; }
+                    slot ^= 1;
+                    if (!slot) sphase ^= 1u;
+                }
+            if (!ok && elect_one()) {       /* what was issued may still run */
+                asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(drain_bar + 8u * h) : "memory");
+                const long long t0 = clock64();
+                while (!mbar_try(drain_bar + 8u * h, 0) && clock64() - t0 < WAIT_CYCLES) { }
+            }
+        }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+        const int quarter = warp & 3, half = (warp - 4) >> 2;       /* this warp's rows and its weight block of the tile's two */
+        const uint32_t lane_base = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(half * 128);
+        const uint32_t tempty0 = leader_addr(tempty_bar(0));
+        float *stg = stage_out + (warp - 4) * 32 * C::STG_PITCH;
+        const int osize = p.out_type == DRK_F32 ? 4 : 2;
+        const bool vec = (reinterpret_cast<uintptr_t>(p.out) % 16 == 0) && (p.ldo * osize % 16 == 0);
+        /* an accumulator is in registers: its slot may be written again */
+        auto release = [&](int a) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster(tempty0 + 8u * a);
+        };
+        drk_dep_wait();
+        int slot = 0;
+        uint32_t sphase = 0;
+        bool ok = true;
+        for (int t = pair; t < tiles && ok; t += pairs) {
+            int mt, nt;
+            place(t, mt, nt);
+            const int row0 = mt * 256 + rank * 128 + quarter * 32;
+            const bool live = row0 + lane < p.n;
+            const int ot = 2 * nt + half;
+            const float4 *sx = reinterpret_cast<const float4 *>(p.sx + (size_t)(live ? row0 + lane : 0) * p.kbp);
+            const float *sw = p.scales + (size_t)(ot < p.ob ? ot : 0) * p.kb;
+            float acc[128];
+#pragma unroll
+            for (int j = 0; j < 128; j++) acc[j] = 0.0f;
+            /* sx of four blocks and of the next four, sw of the next block; the next block's product is made between this one's
+               additions, where its latency costs nothing */
+            float4 now = __ldcg(sx), next = p.kb > 4 ? __ldcg(sx + 1) : now;
+            float s = __ldg(sw + (p.kb > 1)), f = now.x * __ldg(sw);
+            uint32_t ready = mbar_test(tfull_bar(2 * half + slot), sphase);
+            for (int b = 0; b < p.kb; b++) {
+                const uint32_t at = lane_base + (uint32_t)(slot * 256), a = 2 * half + slot;
+                if (!__all_sync(0xffffffffu, ready) && !mbar_wait_warp_inline(tfull_bar(a), sphase, abort_flag, p.status, 44)) { ok = false; break; }
+                tc_fence_after();
+                float f_next = 0.0f;
+#pragma unroll
+                for (int c = 0; c < 2; c++) {
+                    uint32_t r[64];
+                    tmem_ld64(at + 64u * c, r);
+                    if (c == 1) {
+                        release(a);
+                        const int b1 = b + 1;
+                        if ((b1 & 3) == 0) {
+                            now = next;
+                            if (b1 + 4 < p.kb) next = __ldcg(sx + b1 / 4 + 1);
+                        }
+                        f_next = ((b1 & 2) ? ((b1 & 1) ? now.w : now.z) : ((b1 & 1) ? now.y : now.x)) * s;
+                        if (b + 2 < p.kb) s = __ldg(sw + b + 2);
+                        slot ^= 1;
+                        if (!slot) sphase ^= 1u;
+                        ready = mbar_test(tfull_bar(2 * half + slot), sphase);
+                    }
+#pragma unroll
+                    for (int j = 0; j < 64; j++) acc[64 * c + j] = fmaf(f, __uint_as_float(r[j]), acc[64 * c + j]);
+                }
+                f = f_next;
+            }
+            if (!ok) break;
+            /* 32 x 32 at a time through shared memory: a row's 32 outputs are then stored by eight lanes side by side */
+            const int cl = (lane & 7) * 4;
+#pragma unroll
+            for (int c0 = 0; c0 < 128; c0 += 32) {
+                __syncwarp();
+#pragma unroll
+                for (int j = 0; j < 32; j++) stg[lane * C::STG_PITCH + j] = acc[c0 + j];
+                __syncwarp();
+                const int o = ot * FP8_BLOCK + c0 + cl;
+                float bias[4];
+#pragma unroll
+                for (int e = 0; e < 4; e++) bias[e] = p.bias && o + e < p.Nout ? __ldg(p.bias + o + e) : 0.0f;
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const int rr = i * 4 + (lane >> 3);
+                    const size_t r = (size_t)row0 + rr;
+                    if (r >= (size_t)p.n) continue;
+                    float v[4];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) v[e] = fp8_act(stg[rr * C::STG_PITCH + cl + e] + bias[e], p.act);
+                    const size_t at = r * p.ldo + o;
+                    if (vec && o + 4 <= p.Nout) {
+                        if (p.out_type == DRK_F32) *reinterpret_cast<float4 *>(static_cast<float *>(p.out) + at) = make_float4(v[0], v[1], v[2], v[3]);
+                        else {
+                            uint2 w;
+                            if (p.out_type == DRK_BF16) {
+                                const __nv_bfloat162 lo = __floats2bfloat162_rn(v[0], v[1]), hi = __floats2bfloat162_rn(v[2], v[3]);
+                                w = make_uint2(*reinterpret_cast<const uint32_t *>(&lo), *reinterpret_cast<const uint32_t *>(&hi));
+                            } else {
+                                const __half2 lo = __floats2half2_rn(v[0], v[1]), hi = __floats2half2_rn(v[2], v[3]);
+                                w = make_uint2(*reinterpret_cast<const uint32_t *>(&lo), *reinterpret_cast<const uint32_t *>(&hi));
+                            }
+                            *reinterpret_cast<uint2 *>(static_cast<char *>(p.out) + at * 2) = w;
+                        }
+                    } else {
+                        for (int e = 0; e < 4 && o + e < p.Nout; e++) fp8_put(p, r, o + e, v[e]);
+                    }
+                }
+            }
+        }
+    }
+    drk_dep_trigger();
+
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync();     /* neither CTA leaves while the other may still signal it or multiply into its TMEM */
+    if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512) : "memory");
+}
+
 /* ------------------------------------------------------------------ host side */
 typedef CUresult (*PFN_encodeTiled)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
                                     const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -263,39 +616,54 @@ static int encode_rows(CUtensorMap *map, const void *base, size_t rows, int box_
 
 int drk_fp8_tensor_plan(Fp8Tensor *t, const Fp8Params *p, const void *codes, const void *q, int sms)
 {
+    t->pairs = 0;
+    if (p->n > 128) {
+        t->mtiles = (p->n + 255) / 256;
+        t->ntiles = (p->ob + 1) / 2;
+        t->pairs = t->mtiles * t->ntiles < sms / 2 ? t->mtiles * t->ntiles : sms / 2;
+    }
     t->nt = p->n <= 16 ? 16 : p->n <= 32 ? 32 : p->n <= 64 ? 64 : 128;
     const int tiles = p->ob * ((p->n + t->nt - 1) / t->nt);
     t->split = 1;
     while (t->split < 8 && tiles * t->split < sms && t->split * 4 <= p->kb) t->split *= 2;
     /* the attribute holds for the current device, which is the plan's */
-    const cudaError_t e = t->nt == 16   ? cudaFuncSetAttribute(k_fp8_swap<16>, cudaFuncAttributeMaxDynamicSharedMemorySize, SwapCfg<16>::SMEM)
-                          : t->nt == 32 ? cudaFuncSetAttribute(k_fp8_swap<32>, cudaFuncAttributeMaxDynamicSharedMemorySize, SwapCfg<32>::SMEM)
-                          : t->nt == 64 ? cudaFuncSetAttribute(k_fp8_swap<64>, cudaFuncAttributeMaxDynamicSharedMemorySize, SwapCfg<64>::SMEM)
-                                        : cudaFuncSetAttribute(k_fp8_swap<128>, cudaFuncAttributeMaxDynamicSharedMemorySize, SwapCfg<128>::SMEM);
+    const cudaFuncAttribute dyn = cudaFuncAttributeMaxDynamicSharedMemorySize;
+    const cudaError_t e = t->pairs      ? cudaFuncSetAttribute(k_fp8_pair, dyn, PairCfg::SMEM)
+                          : t->nt == 16 ? cudaFuncSetAttribute(k_fp8_swap<16>, dyn, SwapCfg<16>::SMEM)
+                          : t->nt == 32 ? cudaFuncSetAttribute(k_fp8_swap<32>, dyn, SwapCfg<32>::SMEM)
+                          : t->nt == 64 ? cudaFuncSetAttribute(k_fp8_swap<64>, dyn, SwapCfg<64>::SMEM)
+                                        : cudaFuncSetAttribute(k_fp8_swap<128>, dyn, SwapCfg<128>::SMEM);
     if (e != cudaSuccess) return -1;
-    if (encode_rows(&t->mapW, codes, (size_t)p->ob * p->kb * FP8_BLOCK, FP8_BLOCK)) return -1;
+    if (encode_rows(&t->mapW, codes, (size_t)p->ob * p->kb * FP8_BLOCK, t->pairs ? 64 : FP8_BLOCK)) return -1;
     return encode_rows(&t->mapX, q, (size_t)p->kb * p->n, t->nt);
 }
 
-template <int NT> static int swap_launch(cudaStream_t st, const Fp8Tensor *t, const Fp8Params *p)
+template <typename... KArgs, typename... Args>
+static int cluster_launch(void (*kernel)(KArgs...), unsigned grid, unsigned block, unsigned cluster, size_t smem, cudaStream_t st, Args &&...args)
 {
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(p->ob * ((p->n + NT - 1) / NT) * t->split));
-    cfg.blockDim = dim3(192);
-    cfg.dynamicSmemBytes = SwapCfg<NT>::SMEM;
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(block);
+    cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = (unsigned)t->split;
+    attr[0].val.clusterDim.x = cluster;
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = drk_dep_launch_enabled() ? 2 : 1;
-    return drk_launched(cudaLaunchKernelEx(&cfg, k_fp8_swap<NT>, t->mapW, t->mapX, *p, t->split));
+    return drk_launched(cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...));
+}
+
+template <int NT> static int swap_launch(cudaStream_t st, const Fp8Tensor *t, const Fp8Params *p)
+{
+    return cluster_launch(k_fp8_swap<NT>, (unsigned)(p->ob * ((p->n + NT - 1) / NT) * t->split), 192, t->split, SwapCfg<NT>::SMEM, st, t->mapW, t->mapX, *p, t->split);
 }
 
 int drk_fp8_tensor_launch(cudaStream_t st, const Fp8Tensor *t, const Fp8Params *p)
 {
+    if (t->pairs) return cluster_launch(k_fp8_pair, 2u * t->pairs, 384, 2, PairCfg::SMEM, st, t->mapW, t->mapX, *p, t->mtiles, t->ntiles);
     return t->nt == 16 ? swap_launch<16>(st, t, p) : t->nt == 32 ? swap_launch<32>(st, t, p) : t->nt == 64 ? swap_launch<64>(st, t, p) : swap_launch<128>(st, t, p);
 }
