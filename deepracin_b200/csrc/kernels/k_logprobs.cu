@@ -1,11 +1,17 @@
 /*
  * Scoring of a network's outputs: for each row v of `len` logits at temperature 1 / s
  *
- *   lse = log sum_i exp(s v_i),  log p_i = s v_i - lse,  H = -sum_i p_i log p_i = log S - (1 / S) sum_i e_i d_i
+ *   lse = log sum_i exp(s v_i),  log p_i = s v_i - lse,  H = -sum_i p_i log p_i = log S - T / S
  *
- * with d_i = s (v_i - max v), e_i = exp(d_i), S = sum e_i; the log probabilities of given labels, and the k largest logits
- * with their log probabilities.  The order of the alternatives is total: by value (NaN above everything), equal ones by
- * ascending index; a value and its index are compared as one 64-bit key.
+ * with d_i = s (v_i - max v), e_i = exp(d_i), S = sum e_i, T = sum e_i d_i; the log probabilities of given labels, and the k
+ * largest logits with their log probabilities.  The order of the alternatives is total: by value (NaN above everything), equal
+ * ones by ascending index; a value and its index are compared as one 64-bit key, so results do not depend on any timing.
+ *
+ * One pass over the row: each thread holds a running maximum, S and T, rescaled when its maximum grows (d falls by D, so
+ * S -> 2^-D S and T -> 2^-D (T - D S); exponents are kept in base 2), and writes down the maximum of every slot of its share.
+ * The k-th largest of the maxima of 64 groups of threads bounds the k-th largest value from below, so only slots whose maximum
+ * reaches it are read again (for 131072 normal logits and k = 20 about 30 of 4096 slots), and what reaches it is ranked by
+ * counting.  Few rows are split over a cluster of CTAs, which join through distributed shared memory: one launch, no workspace.
  */
 #include <math.h>
 #include <stdio.h>
@@ -13,15 +19,62 @@
 #include <cuda_fp16.h>
 #include "k_common.cuh"
 
-#define LP_THREADS 512
 #define LP_KMAX 32
+#define LP_U 4              /* 16-byte loads a thread has under way, twice (the next batch is requested before this one is used) */
+#define LP_SLOTS 8          /* parts of a thread's share whose maxima are kept */
+#define LP_GROUPS 64
+#define LP_CAND 2048        /* values and slots that a selection may look at; more: a narrower bound, then one pass per alternative */
+#define LP_ITEMS 2048
+#define LP_LOW (-200.0f)    /* 2^-200 is zero in 32 bits: exponents are not held below it, so that no 0 * inf appears */
 
-template <typename T> __device__ __forceinline__ float lp_load(const T *p);
-template <> __device__ __forceinline__ float lp_load(const float *p) { return *p; }
-template <> __device__ __forceinline__ float lp_load(const __nv_bfloat16 *p) { return __bfloat162float(*p); }
-template <> __device__ __forceinline__ float lp_load(const __half *p) { return __half2float(*p); }
+struct LpParams {
+    const void *logits;
+    size_t ld;
+    int len, m, k, split;
+    float scale;
+    const int *labels;
+    float *logprob, *entropy, *top_logprob;
+    int *top_index;
+};
 
-/* float -> uint32 with the order of the values: -inf lowest, +inf below the NaNs, which all map to one value; -0 equals +0 */
+template <typename T> struct LpType;
+template <> struct LpType<float> {
+    static constexpr int V = 4;
+    static constexpr uint32_t FILL = 0xff800000u;
+    static __device__ __forceinline__ float one(const float *p) { return *p; }
+    static __device__ __forceinline__ void unpack(uint4 w, float *v)
+    {
+        v[0] = __uint_as_float(w.x); v[1] = __uint_as_float(w.y); v[2] = __uint_as_float(w.z); v[3] = __uint_as_float(w.w);
+    }
+};
+template <> struct LpType<__nv_bfloat16> {
+    static constexpr int V = 8;
+    static constexpr uint32_t FILL = 0xff80ff80u;
+    static __device__ __forceinline__ float one(const __nv_bfloat16 *p) { return __bfloat162float(*p); }
+    static __device__ __forceinline__ void unpack(uint4 w, float *v)
+    {
+        const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int j = 0; j < 4; j++) { v[2 * j] = __uint_as_float(u[j] << 16); v[2 * j + 1] = __uint_as_float(u[j] & 0xffff0000u); }
+    }
+};
+template <> struct LpType<__half> {
+    static constexpr int V = 8;
+    static constexpr uint32_t FILL = 0xfc00fc00u;
+    static __device__ __forceinline__ float one(const __half *p) { return __half2float(*p); }
+    static __device__ __forceinline__ void unpack(uint4 w, float *v)
+    {
+        const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&u[j]));
+            v[2 * j] = f.x; v[2 * j + 1] = f.y;
+        }
+    }
+};
+
+/* float -> uint32 with the order of the values: -inf lowest, +inf below the NaNs, which all map to one value; -0 equals +0.
+ * 0 stands below every value: nothing there. */
 __device__ __forceinline__ uint32_t lp_order(float v)
 {
     const uint32_t u = __float_as_uint(v + 0.0f);
@@ -29,76 +82,326 @@ __device__ __forceinline__ uint32_t lp_order(float v)
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 __device__ __forceinline__ float lp_value(uint32_t o) { return o == 0xffffffffu ? __uint_as_float(0x7fffffffu) : __uint_as_float(o & 0x80000000u ? o ^ 0x80000000u : ~o); }
-__device__ __forceinline__ unsigned long long lp_key(float v, uint32_t i) { return ((unsigned long long)lp_order(v) << 32) | (0xffffffffu - i); }
+__device__ __forceinline__ unsigned long long lp_key(uint32_t order, uint32_t i) { return ((unsigned long long)order << 32) | (0xffffffffu - i); }
+__device__ __forceinline__ float lp_max_nan(float a, float b) { float r; asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b)); return r; }
+__device__ __forceinline__ float lp_exp2(float x) { float r; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x)); return r; }
 
-__device__ __forceinline__ unsigned long long lp_block_max(unsigned long long v, unsigned long long *red)
+__device__ __forceinline__ float lp_ld_cluster(uint32_t saddr, uint32_t rank)
 {
-    for (int o = 16; o > 0; o >>= 1) {
-        const unsigned long long t = __shfl_xor_sync(0xffffffffu, v, o);
-        v = t > v ? t : v;
+    float v;
+    asm volatile("{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %1, %2;\n\tld.shared::cluster.f32 %0, [a];\n\t}" : "=f"(v) : "r"(saddr), "r"(rank) : "memory");
+    return v;
+}
+__device__ __forceinline__ unsigned long long lp_ld_cluster64(uint32_t saddr, uint32_t rank)
+{
+    unsigned long long v;
+    asm volatile("{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %1, %2;\n\tld.shared::cluster.u64 %0, [a];\n\t}" : "=l"(v) : "r"(saddr), "r"(rank) : "memory");
+    return v;
+}
+__device__ __forceinline__ void lp_cluster_sync()
+{
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+/* S and T of a maximum m, for the maximum `to` >= m */
+__device__ __forceinline__ void lp_rescale(float m, float to, float c, float &S, float &T)
+{
+    if (S > 0.0f) {
+        const float D = fminf((to - m) * c, -LP_LOW), f = lp_exp2(-D);
+        T = f * (T - D * S);
+        S *= f;
     }
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-    __syncthreads();
-    for (int i = 0; i < LP_THREADS / 32; i++) v = red[i] > v ? red[i] : v;
-    return v;
-}
-__device__ __forceinline__ float lp_block_sum(float v, float *red)
-{
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-    __syncthreads();
-    v = 0.0f;
-    for (int i = 0; i < LP_THREADS / 32; i++) v += red[i];
-    return v;
 }
 
-template <typename T>
-__global__ void __launch_bounds__(LP_THREADS) k_logprobs(const T *__restrict__ logits, size_t ld, int len, float s, const int *__restrict__ labels, int m,
-                                                         float *__restrict__ logprob, float *__restrict__ entropy, int k,
-                                                         float *__restrict__ top_logprob, int *__restrict__ top_index)
+template <typename T, int NT>
+__global__ void __launch_bounds__(NT, NT == 512 ? 2 : 8) k_logprobs(const LpParams p)
 {
-    __shared__ unsigned long long red[LP_THREADS / 32];
-    __shared__ float fred[LP_THREADS / 32];
+    using Y = LpType<T>;
+    constexpr int V = Y::V, WARPS = NT / 32, PER_GROUP = NT / LP_GROUPS;
+    __shared__ float smax[LP_SLOTS][NT];
+    __shared__ unsigned long long cand[LP_CAND];
+    __shared__ uint32_t items[LP_ITEMS];
+    __shared__ unsigned long long group[LP_GROUPS], list[LP_KMAX], red[WARPS], bound;
+    __shared__ float fred[3][WARPS];
+    __shared__ float stats[3];              /* this CTA's maximum, S and T */
+    __shared__ uint32_t top_order;          /* order of its largest value, NaN included */
+    __shared__ int n_items, n_cand;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     drk_dep_wait();
     drk_dep_trigger();
-    const size_t row = blockIdx.x;
-    const T *v = logits + row * ld;
-    unsigned long long best = 0;
-    for (int i = threadIdx.x; i < len; i += LP_THREADS) {
-        const unsigned long long key = lp_key(lp_load(v + i), (uint32_t)i);
-        best = key > best ? key : best;
+    const size_t row = blockIdx.x / p.split;
+    const int rank = (int)(blockIdx.x - row * p.split);
+    const T *v = static_cast<const T *>(p.logits) + row * p.ld;
+    /* single values up to the first 16-byte boundary and behind the last one, vectors between them; the cluster shares the vectors */
+    const int head = min(p.len, (int)((16 - (uintptr_t)v % 16) % 16 / sizeof(T)));
+    const int nvec = (p.len - head) / V, singles = rank == 0 ? p.len - nvec * V : 0;
+    const int v0 = (int)((long long)nvec * rank / p.split), count = (int)((long long)nvec * (rank + 1) / p.split) - v0;
+    const uint4 *vec = reinterpret_cast<const uint4 *>(v + head) + v0;
+    const int first = head + v0 * V;        /* index of the share's first value */
+    auto single_index = [&](int i) { return i < head ? i : nvec * V + i; };
+    const float c = p.scale * 1.44269504f;
+    /* the first label's logit is asked for now and used at the end */
+    int label = -1;
+    float labelled = 0.0f;
+    if (rank == 0 && tid < p.m) {
+        label = p.labels[row * p.m + tid];
+        if (label >= 0 && label < p.len) labelled = Y::one(v + label);
     }
-    best = lp_block_max(best, red);
-    const float mx = lp_value((uint32_t)(best >> 32));
-    const float base = mx == -INFINITY ? 0.0f : mx;     /* a row with nothing left: every d_i is -inf */
-    float S = 0.0f, t = 0.0f;
-    for (int i = threadIdx.x; i < len; i += LP_THREADS) {
-        const float d = (lp_load(v + i) - base) * s, e = expf(d);
-        S += e;
-        if (e != 0.0f) t += e * d;
-    }
-    S = lp_block_sum(S, fred);
-    t = lp_block_sum(t, fred);
-    const bool none = mx == -INFINITY;
-    const float ls = logf(S);
-    if (entropy && threadIdx.x == 0) entropy[row] = none ? 0.0f : ls - t / S;
-    for (int j = threadIdx.x; j < m; j += LP_THREADS) {
-        const int l = labels[row * m + j];
-        logprob[row * m + j] = l < 0 ? 0.0f : l >= len ? __uint_as_float(0x7fffffffu) : none ? -INFINITY : (lp_load(v + l) - base) * s - ls;
-    }
-    for (int j = 0; j < k; j++) {
-        if (threadIdx.x == 0) {
-            top_logprob[row * k + j] = none ? -INFINITY : (lp_value((uint32_t)(best >> 32)) - base) * s - ls;
-            top_index[row * k + j] = (int)(0xffffffffu - (uint32_t)best);
+
+    float m = -INFINITY, S0 = 0.0f, S1 = 0.0f, T0 = 0.0f, T1 = 0.0f, mine = -INFINITY;
+    const int batches = (count + NT * LP_U - 1) / (NT * LP_U), per_slot = max(1, (batches + LP_SLOTS - 1) / LP_SLOTS);
+    uint4 next[LP_U];
+    auto fetch = [&](int b) {
+#pragma unroll
+        for (int u = 0; u < LP_U; u++) {
+            const int i = (b * LP_U + u) * NT + tid;
+            next[u] = i < count ? __ldg(vec + i) : make_uint4(Y::FILL, Y::FILL, Y::FILL, Y::FILL);
         }
-        unsigned long long next = 0;
-        for (int i = threadIdx.x; i < len; i += LP_THREADS) {
-            const unsigned long long key = lp_key(lp_load(v + i), (uint32_t)i);
-            if (key < best && key > next) next = key;
+    };
+    if (batches > 0) fetch(0);
+    for (int slot = 0; slot < LP_SLOTS; slot++) {
+        float sm = -INFINITY;
+        for (int b = slot * per_slot; b < min(batches, (slot + 1) * per_slot); b++) {
+            uint4 now[LP_U];
+#pragma unroll
+            for (int u = 0; u < LP_U; u++) now[u] = next[u];
+            if (b + 1 < batches) fetch(b + 1);
+            float bm = -INFINITY;
+#pragma unroll
+            for (int u = 0; u < LP_U; u++) {
+                float x[V];
+                Y::unpack(now[u], x);
+#pragma unroll
+                for (int j = 0; j < V; j++) bm = lp_max_nan(bm, x[j]);
+            }
+            sm = lp_max_nan(sm, bm);
+            if (bm > m) {
+                lp_rescale(m, bm, c, S0, T0);
+                lp_rescale(m, bm, c, S1, T1);
+                m = bm;
+            }
+#pragma unroll
+            for (int u = 0; u < LP_U; u++) {
+                float x[V];
+                Y::unpack(now[u], x);
+#pragma unroll
+                for (int j = 0; j < V; j += 2) {
+                    const float d0 = fmaxf((x[j] - m) * c, LP_LOW), d1 = fmaxf((x[j + 1] - m) * c, LP_LOW);   /* NaN: LP_LOW too */
+                    const float e0 = lp_exp2(d0), e1 = lp_exp2(d1);
+                    S0 += e0; S1 += e1;
+                    T0 = fmaf(e0, d0, T0); T1 = fmaf(e1, d1, T1);
+                }
+            }
         }
-        best = lp_block_max(next, red);
+        smax[slot][tid] = sm;
+        mine = lp_max_nan(mine, sm);
+    }
+    S0 += S1;
+    T0 += T1;
+    uint32_t own_single = 0;                /* order of the single value this thread looks at */
+    if (tid < singles) {
+        const float x = Y::one(v + single_index(tid));
+        own_single = lp_order(x);
+        if (x > m) { lp_rescale(m, x, c, S0, T0); m = x; }
+        const float d = fmaxf((x - m) * c, LP_LOW), e = lp_exp2(d);
+        S0 += e;
+        T0 = fmaf(e, d, T0);
+    }
+    const uint32_t own = tid < count ? lp_order(mine) : 0;      /* order of the largest of this thread's vectors */
+
+    /* the CTA's maximum, S and T */
+    {
+        float M = m;
+        uint32_t O = max(own, own_single);
+        for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+        O = __reduce_max_sync(0xffffffffu, O);
+        if (lane == 0) { fred[0][warp] = M; red[warp] = O; }
+        /* the largest of each group of threads, for the bound below */
+        uint32_t g = own;
+#pragma unroll
+        for (int o = 1; o < PER_GROUP; o <<= 1) g = max(g, __shfl_xor_sync(0xffffffffu, g, o));
+        if (tid % PER_GROUP == 0) group[tid / PER_GROUP] = g;
+        if (tid == 0) { n_items = 0; n_cand = 0; bound = 0; }
+        if (tid < LP_KMAX) list[tid] = 0;
+        __syncthreads();
+        for (int w = 0; w < WARPS; w++) { M = fmaxf(M, fred[0][w]); O = max(O, (uint32_t)red[w]); }
+        lp_rescale(m, M, c, S0, T0);
+        for (int o = 16; o > 0; o >>= 1) { S0 += __shfl_xor_sync(0xffffffffu, S0, o); T0 += __shfl_xor_sync(0xffffffffu, T0, o); }
+        if (lane == 0) { fred[1][warp] = S0; fred[2][warp] = T0; }
+        /* the k-th largest group */
+        if (p.k > 0 && tid < LP_GROUPS) {
+            const uint32_t x = (uint32_t)group[tid];
+            int r = 0;
+            for (int j = 0; j < LP_GROUPS; j++) { const uint32_t y = (uint32_t)group[j]; r += y > x || (y == x && j < tid); }
+            if (r == p.k - 1) bound = (unsigned long long)x << 32;
+        }
+        __syncthreads();
+        if (tid == 0) {
+            float S = 0.0f, T = 0.0f;
+            for (int w = 0; w < WARPS; w++) { S += fred[1][w]; T += fred[2][w]; }
+            stats[0] = M; stats[1] = S; stats[2] = T;
+            top_order = O;
+        }
+    }
+
+    if (p.k > 0) {
+        /* Looks at every value whose key is at least `bound`; false if they or their slots are too many.  A slot's first index
+           bounds the keys of its values that are equal to its maximum. */
+        auto collect = [&]() {
+            const uint32_t border = (uint32_t)(bound >> 32);
+            if (own >= border && own > 0)
+                for (int s = 0; s < LP_SLOTS && s * per_slot < batches; s++)
+                    if (lp_key(lp_order(smax[s][tid]), (uint32_t)(first + (s * per_slot * LP_U * NT + tid) * V)) >= bound) {
+                        const int at = atomicAdd(&n_items, 1);
+                        if (at < LP_ITEMS) items[at] = (uint32_t)tid | ((uint32_t)s << 16);
+                    }
+            auto offer = [&](uint32_t order, int i) {
+                const unsigned long long key = lp_key(order, (uint32_t)i);
+                if (key >= bound) {
+                    const int at = atomicAdd(&n_cand, 1);
+                    if (at < LP_CAND) cand[at] = key;
+                }
+            };
+            if (tid < singles) offer(own_single, single_index(tid));
+            __syncthreads();
+            if (n_items > LP_ITEMS) return false;
+            const int each = per_slot * LP_U;
+            for (int w = tid; w < n_items * each; w += NT) {
+                const uint32_t it = items[w / each];
+                const int i = ((int)(it >> 16) * each + w % each) * NT + (int)(it & 0xffffu);
+                if (i >= count) continue;
+                float x[V];
+                Y::unpack(__ldg(vec + i), x);
+#pragma unroll
+                for (int j = 0; j < V; j++) offer(lp_order(x[j]), first + i * V + j);
+            }
+            __syncthreads();
+            return n_cand <= LP_CAND;
+        };
+        bool ok = collect();
+        if (!ok) {
+            /* Many values equal to the bound (a row of one value, for instance): the same bound on keys, which differ by their
+               index.  A thread's largest stands first in the first slot that has it. */
+            unsigned long long key = 0;
+            if (own > 0) {
+                int s = 0;
+                while (s < LP_SLOTS - 1 && lp_order(smax[s][tid]) != own) s++;
+                for (int w = 0; w < per_slot * LP_U && key == 0; w++) {
+                    const int i = (s * per_slot * LP_U + w) * NT + tid;
+                    if (i >= count) break;
+                    float x[V];
+                    Y::unpack(__ldg(vec + i), x);
+                    for (int j = V - 1; j >= 0; j--) if (lp_order(x[j]) == own) key = lp_key(own, (uint32_t)(first + i * V + j));
+                }
+            }
+#pragma unroll
+            for (int o = 1; o < PER_GROUP; o <<= 1) {
+                const unsigned long long y = __shfl_xor_sync(0xffffffffu, key, o);
+                key = y > key ? y : key;
+            }
+            __syncthreads();
+            if (tid % PER_GROUP == 0) group[tid / PER_GROUP] = key;
+            if (tid == 0) { n_items = 0; n_cand = 0; }
+            __syncthreads();
+            if (tid < LP_GROUPS) {
+                const unsigned long long x = group[tid];
+                int r = 0;
+                for (int j = 0; j < LP_GROUPS; j++) r += group[j] > x || (group[j] == x && j < tid);
+                if (r == p.k - 1) bound = x;
+            }
+            __syncthreads();
+            ok = collect();
+        }
+        if (ok) {
+            for (int i = tid; i < n_cand; i += NT) {
+                const unsigned long long key = cand[i];
+                int r = 0;
+                for (int j = 0; j < n_cand; j++) r += cand[j] > key;
+                if (r < p.k) list[r] = key;
+            }
+        } else {
+            /* the largest values crowd in few threads' shares: one pass over the row for each alternative */
+            unsigned long long last = ~0ull;
+            for (int r = 0; r < p.k; r++) {
+                unsigned long long best = 0;
+                for (int i = tid; i < count; i += NT) {
+                    float x[V];
+                    Y::unpack(__ldg(vec + i), x);
+#pragma unroll
+                    for (int j = 0; j < V; j++) {
+                        const unsigned long long key = lp_key(lp_order(x[j]), (uint32_t)(first + i * V + j));
+                        if (key < last && key > best) best = key;
+                    }
+                }
+                if (tid < singles) {
+                    const unsigned long long key = lp_key(own_single, (uint32_t)single_index(tid));
+                    if (key < last && key > best) best = key;
+                }
+                for (int o = 16; o > 0; o >>= 1) {
+                    const unsigned long long y = __shfl_xor_sync(0xffffffffu, best, o);
+                    best = y > best ? y : best;
+                }
+                __syncthreads();
+                if (lane == 0) red[warp] = best;
+                __syncthreads();
+                for (int w = 0; w < WARPS; w++) best = red[w] > best ? red[w] : best;
+                if (tid == 0) list[r] = best;
+                last = best;
+            }
+        }
+    }
+    __syncthreads();
+
+    float M = stats[0], S = stats[1], E = stats[2];
+    uint32_t O = top_order;
+    if (p.split > 1) {
+        lp_cluster_sync();
+        if (rank == 0) {
+            const uint32_t at = (uint32_t)__cvta_generic_to_shared(stats), lat = (uint32_t)__cvta_generic_to_shared(list);
+            const uint32_t oat = (uint32_t)__cvta_generic_to_shared(&top_order);
+            for (int r = 1; r < p.split; r++) {
+                M = fmaxf(M, lp_ld_cluster(at, r));
+                O = max(O, __float_as_uint(lp_ld_cluster(oat, r)));
+            }
+            S = E = 0.0f;
+            for (int r = 0; r < p.split; r++) {
+                float s = lp_ld_cluster(at + 4, r), t = lp_ld_cluster(at + 8, r);
+                lp_rescale(lp_ld_cluster(at, r), M, c, s, t);
+                S += s;
+                E += t;
+            }
+            const int all = p.split * LP_KMAX;
+            if (p.k > 0) for (int i = tid; i < all; i += NT) cand[i] = lp_ld_cluster64(lat + 8 * (i % LP_KMAX), i / LP_KMAX);
+        }
+        lp_cluster_sync();      /* what the others hold has been read */
+        if (rank != 0) return;
+        const int all = p.split * LP_KMAX;
+        if (p.k > 0)
+            for (int i = tid; i < all; i += NT) {
+                const unsigned long long key = cand[i];
+                int r = 0;
+                for (int j = 0; j < all; j++) r += cand[j] > key;
+                if (key != 0 && r < p.k) list[r] = key;
+            }
+        __syncthreads();
+    }
+
+    const bool none = M == -INFINITY && O == lp_order(-INFINITY), bad = O >= lp_order(INFINITY);
+    const float nan = __uint_as_float(0x7fffffffu), logS = logf(S);
+    auto score = [&](float x) { return bad ? nan : none || x == -INFINITY ? -INFINITY : (x - M) * p.scale - logS; };
+    if (p.entropy && tid == 0) p.entropy[row] = bad ? nan : none ? 0.0f : logS - E / S * 0.693147181f;
+    for (int j = tid; j < p.m; j += NT) {
+        if (j != tid) {
+            label = p.labels[row * p.m + j];
+            if (label >= 0 && label < p.len) labelled = Y::one(v + label);
+        }
+        p.logprob[row * p.m + j] = label < 0 ? 0.0f : label >= p.len ? nan : score(labelled);
+    }
+    for (int j = tid; j < p.k; j += NT) {
+        const unsigned long long key = list[j];
+        p.top_logprob[row * p.k + j] = score(lp_value((uint32_t)(key >> 32)));
+        p.top_index[row * p.k + j] = (int)(0xffffffffu - (uint32_t)key);
     }
 }
 
@@ -108,12 +411,37 @@ static int lp_refuse(const char *why)
     return -1;
 }
 
-template <typename T>
-static cudaError_t lp_launch(cudaStream_t st, const void *logits, size_t ld, int n, int len, float scale, const int *labels, int m, float *logprob,
-                             float *entropy, int k, float *top_logprob, int *top_index)
+template <typename T, int NT> static int lp_launch(cudaStream_t st, const LpParams &p, int n)
 {
-    return drk_launch_dep(k_logprobs<T>, dim3((unsigned)n), dim3(LP_THREADS), 0, st, (const T *)logits, ld, len, scale, labels, m, logprob, entropy, k,
-                          top_logprob, top_index);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)n * (unsigned)p.split);
+    cfg.blockDim = dim3(NT);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    int na = 0;
+    if (p.split > 1) {
+        attr[na].id = cudaLaunchAttributeClusterDimension;
+        attr[na].val.clusterDim.x = (unsigned)p.split;
+        attr[na].val.clusterDim.y = attr[na].val.clusterDim.z = 1;
+        na++;
+    }
+    if (drk_dep_launch_enabled()) {
+        attr[na].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[na].val.programmaticStreamSerializationAllowed = 1;
+        na++;
+    }
+    cfg.attrs = attr;
+    cfg.numAttrs = na;
+    return drk_launched(cudaLaunchKernelEx(&cfg, k_logprobs<T, NT>, p));
+}
+
+/* Rows are split over a cluster until there are two CTAs for every SM, as long as a share keeps a batch of loads for each of its
+ * threads; shares of at most one batch of 128 threads run with 128. */
+template <typename T> static int lp_run(cudaStream_t st, LpParams &p, int n)
+{
+    constexpr int V = LpType<T>::V;
+    while (p.split < 8 && (long long)n * p.split < 2 * 148 && p.len / (2 * p.split) >= 512 * V) p.split *= 2;
+    return p.len / p.split <= 128 * LP_U * V ? lp_launch<T, 128>(st, p, n) : lp_launch<T, 512>(st, p, n);
 }
 
 extern "C" int dRk_logprobs(dRk_stream stream, const void *logits, int type, long long ld, int n, int len, float scale, const int *labels, int m,
@@ -122,6 +450,7 @@ extern "C" int dRk_logprobs(dRk_stream stream, const void *logits, int type, lon
     const int size = type == DRK_F32 ? 4 : type == DRK_BF16 || type == DRK_F16 ? 2 : 0;
     if (!size) return lp_refuse("unknown element type");
     if (n < 1 || len < 1) return lp_refuse("needs at least one row and one logit");
+    if (n > 1 << 28 || len > 1 << 30) return lp_refuse("more than 2^28 rows or 2^30 logits");
     if (n > 1 && ld < len) return lp_refuse("rows overlap (ld < len)");
     if (m < 0 || k < 0 || k > LP_KMAX || k > len) return lp_refuse("number of labels below 0, or of alternatives outside 0..min(32, len)");
     if (!logits || (m > 0 && (!labels || !logprob)) || (k > 0 && (!top_logprob || !top_index))) return lp_refuse("null pointer");
@@ -130,10 +459,14 @@ extern "C" int dRk_logprobs(dRk_stream stream, const void *logits, int type, lon
         return lp_refuse("pointer not aligned to its element type");
     const int dev = drk_stream_device("dRk_logprobs", stream, -1);
     if (dev < 0) return dev;
+    LpParams p = {};
+    p.logits = logits;
+    p.ld = n > 1 ? (size_t)ld : 0;
+    p.len = len; p.m = m; p.k = k; p.split = 1;
+    p.scale = scale;
+    p.labels = labels;
+    p.logprob = logprob; p.entropy = entropy;
+    p.top_logprob = top_logprob; p.top_index = top_index;
     cudaStream_t st = drk_stream(stream);
-    const size_t pitch = n > 1 ? (size_t)ld : 0;
-    const cudaError_t e = type == DRK_F32    ? lp_launch<float>(st, logits, pitch, n, len, scale, labels, m, logprob, entropy, k, top_logprob, top_index)
-                          : type == DRK_BF16 ? lp_launch<__nv_bfloat16>(st, logits, pitch, n, len, scale, labels, m, logprob, entropy, k, top_logprob, top_index)
-                                             : lp_launch<__half>(st, logits, pitch, n, len, scale, labels, m, logprob, entropy, k, top_logprob, top_index);
-    return drk_launched(e);
+    return type == DRK_F32 ? lp_run<float>(st, p, n) : type == DRK_BF16 ? lp_run<__nv_bfloat16>(st, p, n) : lp_run<__half>(st, p, n);
 }
