@@ -63,9 +63,11 @@ static inline int drk_stream_device(const char *who, dRk_stream stream, int want
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess) { (void)cudaGetLastError(); fprintf(stderr, "%s: no CUDA device\n", who); return -5; }
     int sdev = dev;
-    cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
-    if (cudaStreamIsCapturing(drk_stream(stream), &capturing) != cudaSuccess) { (void)cudaGetLastError(); capturing = cudaStreamCaptureStatusActive; }
-    if (capturing == cudaStreamCaptureStatusNone && cudaStreamGetDevice(drk_stream(stream), &sdev) != cudaSuccess) { (void)cudaGetLastError(); sdev = dev; }
+    if (stream) {       /* the default stream is the current device's */
+        cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
+        if (cudaStreamIsCapturing(drk_stream(stream), &capturing) != cudaSuccess) { (void)cudaGetLastError(); capturing = cudaStreamCaptureStatusActive; }
+        if (capturing == cudaStreamCaptureStatusNone && cudaStreamGetDevice(drk_stream(stream), &sdev) != cudaSuccess) { (void)cudaGetLastError(); sdev = dev; }
+    }
     if (sdev != dev || (want >= 0 && want != dev)) {
         fprintf(stderr, "%s: device %d is current, the stream belongs to device %d%s\n", who, dev, sdev,
                 want >= 0 && want != dev ? " and the plan to another one" : "");

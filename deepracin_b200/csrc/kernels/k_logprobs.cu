@@ -12,6 +12,12 @@
  * The k-th largest of the maxima of 64 groups of threads bounds the k-th largest value from below, so only slots whose maximum
  * reaches it are read again (for 131072 normal logits and k = 20 about 30 of 4096 slots), and what reaches it is ranked by
  * counting.  Few rows are split over a cluster of CTAs, which join through distributed shared memory: one launch, no workspace.
+ *
+ * Bound by HBM in 32 bits (2048 x 131072: 163 us without alternatives = 6.6 TB/s, 178 us with five, 184 us with twenty) and by the
+ * issue of about eight instructions a value in 16 bits (1024 x 131072 bf16: 56 and 61 us, 41 us at the copy rate); below that by the
+ * chain of a launch, one round of loads and the selection's barriers (1 x 1000: 2.7 us, 4.6 us with five; 1 x 131072 bf16: 4.3 and
+ * 8.2 us with twenty).  CTAs of 512 threads instead of 256 took 192 us and 35 instead of 24 us for 1000 x 32000: with two of them
+ * on an SM half its loads stop during a selection.  d as one FMA, x c - m c, saved nothing and left a row of one value off zero.
  */
 #include <math.h>
 #include <stdio.h>
@@ -20,6 +26,9 @@
 #include "k_common.cuh"
 
 #define LP_KMAX 32
+#define LP_LN2 0.693147181f
+#define LP_NT 256           /* threads of a CTA, four of which share an SM */
+#define LP_SPLIT 8          /* CTAs that share a row at most */
 #define LP_U 4              /* 16-byte loads a thread has under way, twice (the next batch is requested before this one is used) */
 #define LP_SLOTS 8          /* parts of a thread's share whose maxima are kept */
 #define LP_GROUPS 64
@@ -37,10 +46,16 @@ struct LpParams {
     int *top_index;
 };
 
+/* the larger one, NaN if either is */
+__device__ __forceinline__ float lp_max_nan(float a, float b) { float r; asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b)); return r; }
+
+/* a 16-byte load of each type; max2: the larger of packed values, last: the larger of what a word holds */
 template <typename T> struct LpType;
 template <> struct LpType<float> {
     static constexpr int V = 4;
     static constexpr uint32_t FILL = 0xff800000u;
+    static __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) { uint32_t r; asm("max.NaN.f32 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b)); return r; }
+    static __device__ __forceinline__ float last(uint32_t a) { return __uint_as_float(a); }
     static __device__ __forceinline__ float one(const float *p) { return *p; }
     static __device__ __forceinline__ void unpack(uint4 w, float *v)
     {
@@ -50,6 +65,8 @@ template <> struct LpType<float> {
 template <> struct LpType<__nv_bfloat16> {
     static constexpr int V = 8;
     static constexpr uint32_t FILL = 0xff80ff80u;
+    static __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) { uint32_t r; asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b)); return r; }
+    static __device__ __forceinline__ float last(uint32_t a) { return lp_max_nan(__uint_as_float(a << 16), __uint_as_float(a & 0xffff0000u)); }
     static __device__ __forceinline__ float one(const __nv_bfloat16 *p) { return __bfloat162float(*p); }
     static __device__ __forceinline__ void unpack(uint4 w, float *v)
     {
@@ -61,6 +78,12 @@ template <> struct LpType<__nv_bfloat16> {
 template <> struct LpType<__half> {
     static constexpr int V = 8;
     static constexpr uint32_t FILL = 0xfc00fc00u;
+    static __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) { uint32_t r; asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b)); return r; }
+    static __device__ __forceinline__ float last(uint32_t a)
+    {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&a));
+        return lp_max_nan(f.x, f.y);
+    }
     static __device__ __forceinline__ float one(const __half *p) { return __half2float(*p); }
     static __device__ __forceinline__ void unpack(uint4 w, float *v)
     {
@@ -83,51 +106,59 @@ __device__ __forceinline__ uint32_t lp_order(float v)
 }
 __device__ __forceinline__ float lp_value(uint32_t o) { return o == 0xffffffffu ? __uint_as_float(0x7fffffffu) : __uint_as_float(o & 0x80000000u ? o ^ 0x80000000u : ~o); }
 __device__ __forceinline__ unsigned long long lp_key(uint32_t order, uint32_t i) { return ((unsigned long long)order << 32) | (0xffffffffu - i); }
-__device__ __forceinline__ float lp_max_nan(float a, float b) { float r; asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b)); return r; }
 __device__ __forceinline__ float lp_exp2(float x) { float r; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x)); return r; }
 
-__device__ __forceinline__ float lp_ld_cluster(uint32_t saddr, uint32_t rank)
+/* stores into the shared memory of the cluster's CTA 0 */
+__device__ __forceinline__ void lp_st_first(uint32_t saddr, float v)
 {
-    float v;
-    asm volatile("{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %1, %2;\n\tld.shared::cluster.f32 %0, [a];\n\t}" : "=f"(v) : "r"(saddr), "r"(rank) : "memory");
-    return v;
+    asm volatile("{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %0, 0;\n\tst.shared::cluster.f32 [a], %1;\n\t}" ::"r"(saddr), "f"(v) : "memory");
 }
-__device__ __forceinline__ unsigned long long lp_ld_cluster64(uint32_t saddr, uint32_t rank)
+__device__ __forceinline__ void lp_st_first(uint32_t saddr, unsigned long long v)
 {
-    unsigned long long v;
-    asm volatile("{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %1, %2;\n\tld.shared::cluster.u64 %0, [a];\n\t}" : "=l"(v) : "r"(saddr), "r"(rank) : "memory");
-    return v;
+    asm volatile("{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %0, 0;\n\tst.shared::cluster.u64 [a], %1;\n\t}" ::"r"(saddr), "l"(v) : "memory");
 }
-__device__ __forceinline__ void lp_cluster_sync()
+__device__ __forceinline__ void lp_cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void lp_cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+
+/* how many of n keys are larger */
+__device__ __forceinline__ int lp_rank(const unsigned long long *keys, int n, unsigned long long key)
 {
-    __syncwarp();
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    int r = 0;
+#pragma unroll 4
+    for (int j = 0; j < n; j += 2) {
+        const ulonglong2 y = *reinterpret_cast<const ulonglong2 *>(keys + j);
+        r += (y.x > key) + (j + 1 < n && y.y > key);
+    }
+    return r;
 }
 
-/* S and T of a maximum m, for the maximum `to` >= m */
-__device__ __forceinline__ void lp_rescale(float m, float to, float c, float &S, float &T)
+/* S and T after the maximum grew by D (in base 2, times the scale) */
+__device__ __forceinline__ void lp_rescale(float D, float &S, float &T)
 {
     if (S > 0.0f) {
-        const float D = fminf((to - m) * c, -LP_LOW), f = lp_exp2(-D);
+        D = fminf(D, -LP_LOW);
+        const float f = lp_exp2(-D);
         T = f * (T - D * S);
         S *= f;
     }
 }
 
 template <typename T, int NT>
-__global__ void __launch_bounds__(NT, NT == 512 ? 2 : 8) k_logprobs(const LpParams p)
+__global__ void __launch_bounds__(NT, 1024 / NT) k_logprobs(const LpParams p)
 {
     using Y = LpType<T>;
     constexpr int V = Y::V, WARPS = NT / 32, PER_GROUP = NT / LP_GROUPS;
     __shared__ float smax[LP_SLOTS][NT];
-    __shared__ unsigned long long cand[LP_CAND];
+    __shared__ __align__(16) unsigned long long cand[LP_CAND + 2];
+    __shared__ __align__(16) unsigned long long all[LP_SPLIT * LP_KMAX];    /* the alternatives of the cluster's CTAs, k each */
+    __shared__ float stats[LP_SPLIT][4];    /* their maxima, S, T and the orders of their largest values (NaN included) */
     __shared__ uint32_t items[LP_ITEMS];
-    __shared__ unsigned long long group[LP_GROUPS], list[LP_KMAX], red[WARPS], bound;
-    __shared__ float fred[3][WARPS];
-    __shared__ float stats[3];              /* this CTA's maximum, S and T */
-    __shared__ uint32_t top_order;          /* order of its largest value, NaN included */
+    __shared__ unsigned long long group_key[LP_GROUPS], list[LP_KMAX], red[WARPS], bound;
+    __shared__ __align__(16) uint32_t group[LP_GROUPS];
+    __shared__ float fred[4][WARPS];
     __shared__ int n_items, n_cand;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    if (p.split > 1) lp_cluster_arrive();   /* waited for before the first store into another CTA: it runs by then */
     drk_dep_wait();
     drk_dep_trigger();
     const size_t row = blockIdx.x / p.split;
@@ -167,18 +198,15 @@ __global__ void __launch_bounds__(NT, NT == 512 ? 2 : 8) k_logprobs(const LpPara
 #pragma unroll
             for (int u = 0; u < LP_U; u++) now[u] = next[u];
             if (b + 1 < batches) fetch(b + 1);
-            float bm = -INFINITY;
+            uint32_t w2 = Y::max2(now[0].x, now[0].y);
+            w2 = Y::max2(w2, Y::max2(now[0].z, now[0].w));
 #pragma unroll
-            for (int u = 0; u < LP_U; u++) {
-                float x[V];
-                Y::unpack(now[u], x);
-#pragma unroll
-                for (int j = 0; j < V; j++) bm = lp_max_nan(bm, x[j]);
-            }
+            for (int u = 1; u < LP_U; u++) w2 = Y::max2(w2, Y::max2(Y::max2(now[u].x, now[u].y), Y::max2(now[u].z, now[u].w)));
+            const float bm = Y::last(w2);
             sm = lp_max_nan(sm, bm);
             if (bm > m) {
-                lp_rescale(m, bm, c, S0, T0);
-                lp_rescale(m, bm, c, S1, T1);
+                lp_rescale((bm - m) * c, S0, T0);
+                lp_rescale((bm - m) * c, S1, T1);
                 m = bm;
             }
 #pragma unroll
@@ -187,7 +215,7 @@ __global__ void __launch_bounds__(NT, NT == 512 ? 2 : 8) k_logprobs(const LpPara
                 Y::unpack(now[u], x);
 #pragma unroll
                 for (int j = 0; j < V; j += 2) {
-                    const float d0 = fmaxf((x[j] - m) * c, LP_LOW), d1 = fmaxf((x[j + 1] - m) * c, LP_LOW);   /* NaN: LP_LOW too */
+                    const float d0 = fmaxf((x[j] - m) * c, LP_LOW), d1 = fmaxf((x[j + 1] - m) * c, LP_LOW);    /* NaN: LP_LOW too */
                     const float e0 = lp_exp2(d0), e1 = lp_exp2(d1);
                     S0 += e0; S1 += e1;
                     T0 = fmaf(e0, d0, T0); T1 = fmaf(e1, d1, T1);
@@ -203,7 +231,10 @@ __global__ void __launch_bounds__(NT, NT == 512 ? 2 : 8) k_logprobs(const LpPara
     if (tid < singles) {
         const float x = Y::one(v + single_index(tid));
         own_single = lp_order(x);
-        if (x > m) { lp_rescale(m, x, c, S0, T0); m = x; }
+        if (x > m) {
+            lp_rescale((x - m) * c, S0, T0);
+            m = x;
+        }
         const float d = fmaxf((x - m) * c, LP_LOW), e = lp_exp2(d);
         S0 += e;
         T0 = fmaf(e, d, T0);
@@ -211,51 +242,45 @@ __global__ void __launch_bounds__(NT, NT == 512 ? 2 : 8) k_logprobs(const LpPara
     const uint32_t own = tid < count ? lp_order(mine) : 0;      /* order of the largest of this thread's vectors */
 
     /* the CTA's maximum, S and T */
-    {
-        float M = m;
-        uint32_t O = max(own, own_single);
-        for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-        O = __reduce_max_sync(0xffffffffu, O);
-        if (lane == 0) { fred[0][warp] = M; red[warp] = O; }
-        /* the largest of each group of threads, for the bound below */
-        uint32_t g = own;
+    float M = m, S = 0.0f, E = 0.0f;
+    uint32_t O = __reduce_max_sync(0xffffffffu, max(own, own_single));
+    for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+    if (lane == 0) { fred[0][warp] = M; fred[1][warp] = __uint_as_float(O); }
+    /* the largest of each group of threads, for the bound below */
+    uint32_t g = own;
 #pragma unroll
-        for (int o = 1; o < PER_GROUP; o <<= 1) g = max(g, __shfl_xor_sync(0xffffffffu, g, o));
-        if (tid % PER_GROUP == 0) group[tid / PER_GROUP] = g;
-        if (tid == 0) { n_items = 0; n_cand = 0; bound = 0; }
-        if (tid < LP_KMAX) list[tid] = 0;
-        __syncthreads();
-        for (int w = 0; w < WARPS; w++) { M = fmaxf(M, fred[0][w]); O = max(O, (uint32_t)red[w]); }
-        lp_rescale(m, M, c, S0, T0);
-        for (int o = 16; o > 0; o >>= 1) { S0 += __shfl_xor_sync(0xffffffffu, S0, o); T0 += __shfl_xor_sync(0xffffffffu, T0, o); }
-        if (lane == 0) { fred[1][warp] = S0; fred[2][warp] = T0; }
-        /* the k-th largest group */
-        if (p.k > 0 && tid < LP_GROUPS) {
-            const uint32_t x = (uint32_t)group[tid];
-            int r = 0;
-            for (int j = 0; j < LP_GROUPS; j++) { const uint32_t y = (uint32_t)group[j]; r += y > x || (y == x && j < tid); }
-            if (r == p.k - 1) bound = (unsigned long long)x << 32;
+    for (int o = 1; o < PER_GROUP; o <<= 1) g = max(g, __shfl_xor_sync(0xffffffffu, g, o));
+    if (tid % PER_GROUP == 0) group[tid / PER_GROUP] = g;
+    if (tid == 0) { n_items = 0; n_cand = 0; bound = 0; }
+    if (tid < LP_KMAX) list[tid] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < WARPS; w++) { M = fmaxf(M, fred[0][w]); O = max(O, __float_as_uint(fred[1][w])); }
+    lp_rescale((M - m) * c, S0, T0);
+    for (int o = 16; o > 0; o >>= 1) { S0 += __shfl_xor_sync(0xffffffffu, S0, o); T0 += __shfl_xor_sync(0xffffffffu, T0, o); }
+    if (lane == 0) { fred[2][warp] = S0; fred[3][warp] = T0; }
+    /* the k-th largest group */
+    if (p.k > 0 && tid < LP_GROUPS) {
+        const uint32_t x = group[tid];
+        int r = 0;
+#pragma unroll
+        for (int j = 0; j < LP_GROUPS; j += 4) {
+            const uint4 y = *reinterpret_cast<const uint4 *>(group + j);
+            r += (y.x > x || (y.x == x && j < tid)) + (y.y > x || (y.y == x && j + 1 < tid)) + (y.z > x || (y.z == x && j + 2 < tid)) +
+                 (y.w > x || (y.w == x && j + 3 < tid));
         }
-        __syncthreads();
-        if (tid == 0) {
-            float S = 0.0f, T = 0.0f;
-            for (int w = 0; w < WARPS; w++) { S += fred[1][w]; T += fred[2][w]; }
-            stats[0] = M; stats[1] = S; stats[2] = T;
-            top_order = O;
-        }
+        if (r == p.k - 1) bound = (unsigned long long)x << 32;
     }
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < WARPS; w++) { S += fred[2][w]; E += fred[3][w]; }
 
     if (p.k > 0) {
         /* Looks at every value whose key is at least `bound`; false if they or their slots are too many.  A slot's first index
            bounds the keys of its values that are equal to its maximum. */
         auto collect = [&]() {
             const uint32_t border = (uint32_t)(bound >> 32);
-            if (own >= border && own > 0)
-                for (int s = 0; s < LP_SLOTS && s * per_slot < batches; s++)
-                    if (lp_key(lp_order(smax[s][tid]), (uint32_t)(first + (s * per_slot * LP_U * NT + tid) * V)) >= bound) {
-                        const int at = atomicAdd(&n_items, 1);
-                        if (at < LP_ITEMS) items[at] = (uint32_t)tid | ((uint32_t)s << 16);
-                    }
+            const float low = lp_value(border);         /* NaN where everything counts: x < low is false then */
             auto offer = [&](uint32_t order, int i) {
                 const unsigned long long key = lp_key(order, (uint32_t)i);
                 if (key >= bound) {
@@ -264,6 +289,12 @@ __global__ void __launch_bounds__(NT, NT == 512 ? 2 : 8) k_logprobs(const LpPara
                 }
             };
             if (tid < singles) offer(own_single, single_index(tid));
+            if (own >= border && own > 0)
+                for (int s = 0; s < LP_SLOTS && s * per_slot < batches; s++)
+                    if (lp_key(lp_order(smax[s][tid]), (uint32_t)(first + (s * per_slot * LP_U * NT + tid) * V)) >= bound) {
+                        const int at = atomicAdd(&n_items, 1);
+                        if (at < LP_ITEMS) items[at] = (uint32_t)tid | ((uint32_t)s << 16);
+                    }
             __syncthreads();
             if (n_items > LP_ITEMS) return false;
             const int each = per_slot * LP_U;
@@ -274,7 +305,7 @@ __global__ void __launch_bounds__(NT, NT == 512 ? 2 : 8) k_logprobs(const LpPara
                 float x[V];
                 Y::unpack(__ldg(vec + i), x);
 #pragma unroll
-                for (int j = 0; j < V; j++) offer(lp_order(x[j]), first + i * V + j);
+                for (int j = 0; j < V; j++) if (!(x[j] < low)) offer(lp_order(x[j]), first + i * V + j);
             }
             __syncthreads();
             return n_cand <= LP_CAND;
@@ -301,23 +332,23 @@ __global__ void __launch_bounds__(NT, NT == 512 ? 2 : 8) k_logprobs(const LpPara
                 key = y > key ? y : key;
             }
             __syncthreads();
-            if (tid % PER_GROUP == 0) group[tid / PER_GROUP] = key;
+            if (tid % PER_GROUP == 0) group_key[tid / PER_GROUP] = key;
             if (tid == 0) { n_items = 0; n_cand = 0; }
             __syncthreads();
             if (tid < LP_GROUPS) {
-                const unsigned long long x = group[tid];
+                const unsigned long long x = group_key[tid];
                 int r = 0;
-                for (int j = 0; j < LP_GROUPS; j++) r += group[j] > x || (group[j] == x && j < tid);
+                for (int j = 0; j < LP_GROUPS; j++) r += group_key[j] > x || (group_key[j] == x && j < tid);
                 if (r == p.k - 1) bound = x;
             }
             __syncthreads();
             ok = collect();
         }
         if (ok) {
-            for (int i = tid; i < n_cand; i += NT) {
+            const int n = n_cand;
+            for (int i = tid; i < n; i += NT) {
                 const unsigned long long key = cand[i];
-                int r = 0;
-                for (int j = 0; j < n_cand; j++) r += cand[j] > key;
+                const int r = lp_rank(cand, n, key);
                 if (r < p.k) list[r] = key;
             }
         } else {
@@ -353,44 +384,39 @@ __global__ void __launch_bounds__(NT, NT == 512 ? 2 : 8) k_logprobs(const LpPara
     }
     __syncthreads();
 
-    float M = stats[0], S = stats[1], E = stats[2];
-    uint32_t O = top_order;
     if (p.split > 1) {
-        lp_cluster_sync();
-        if (rank == 0) {
-            const uint32_t at = (uint32_t)__cvta_generic_to_shared(stats), lat = (uint32_t)__cvta_generic_to_shared(list);
-            const uint32_t oat = (uint32_t)__cvta_generic_to_shared(&top_order);
-            for (int r = 1; r < p.split; r++) {
-                M = fmaxf(M, lp_ld_cluster(at, r));
-                O = max(O, __float_as_uint(lp_ld_cluster(oat, r)));
-            }
-            S = E = 0.0f;
-            for (int r = 0; r < p.split; r++) {
-                float s = lp_ld_cluster(at + 4, r), t = lp_ld_cluster(at + 8, r);
-                lp_rescale(lp_ld_cluster(at, r), M, c, s, t);
+        __syncwarp();
+        lp_cluster_wait();
+        if (tid < p.k) lp_st_first((uint32_t)__cvta_generic_to_shared(all + rank * p.k + tid), list[tid]);
+        if (tid < 4) lp_st_first((uint32_t)__cvta_generic_to_shared(&stats[rank][tid]), tid == 0 ? M : tid == 1 ? S : tid == 2 ? E : __uint_as_float(O));
+        __syncwarp();
+        lp_cluster_arrive();
+        if (rank != 0) return;
+        lp_cluster_wait();
+        S = E = 0.0f;
+#pragma unroll
+        for (int r = 0; r < LP_SPLIT; r++)
+            if (r < p.split) { M = fmaxf(M, stats[r][0]); O = max(O, __float_as_uint(stats[r][3])); }
+#pragma unroll
+        for (int r = 0; r < LP_SPLIT; r++)
+            if (r < p.split) {
+                float s = stats[r][1], t = stats[r][2];
+                lp_rescale((M - stats[r][0]) * c, s, t);
                 S += s;
                 E += t;
             }
-            const int all = p.split * LP_KMAX;
-            if (p.k > 0) for (int i = tid; i < all; i += NT) cand[i] = lp_ld_cluster64(lat + 8 * (i % LP_KMAX), i / LP_KMAX);
+        for (int i = tid; i < p.split * p.k; i += NT) {
+            const unsigned long long key = all[i];
+            const int r = lp_rank(all, p.split * p.k, key);
+            if (key != 0 && r < p.k) list[r] = key;
         }
-        lp_cluster_sync();      /* what the others hold has been read */
-        if (rank != 0) return;
-        const int all = p.split * LP_KMAX;
-        if (p.k > 0)
-            for (int i = tid; i < all; i += NT) {
-                const unsigned long long key = cand[i];
-                int r = 0;
-                for (int j = 0; j < all; j++) r += cand[j] > key;
-                if (key != 0 && r < p.k) list[r] = key;
-            }
         __syncthreads();
     }
 
     const bool none = M == -INFINITY && O == lp_order(-INFINITY), bad = O >= lp_order(INFINITY);
     const float nan = __uint_as_float(0x7fffffffu), logS = logf(S);
     auto score = [&](float x) { return bad ? nan : none || x == -INFINITY ? -INFINITY : (x - M) * p.scale - logS; };
-    if (p.entropy && tid == 0) p.entropy[row] = bad ? nan : none ? 0.0f : logS - E / S * 0.693147181f;
+    if (p.entropy && tid == 0) p.entropy[row] = bad ? nan : none ? 0.0f : logS - E / S * LP_LN2;
     for (int j = tid; j < p.m; j += NT) {
         if (j != tid) {
             label = p.labels[row * p.m + j];
@@ -435,13 +461,17 @@ template <typename T, int NT> static int lp_launch(cudaStream_t st, const LpPara
     return drk_launched(cudaLaunchKernelEx(&cfg, k_logprobs<T, NT>, p));
 }
 
-/* Rows are split over a cluster until there are two CTAs for every SM, as long as a share keeps a batch of loads for each of its
- * threads; shares of at most one batch of 128 threads run with 128. */
+/* A row is split over up to eight CTAs while that leaves at most two on each of 148 SMs and a load for each thread of a share.
+ * Four would fit, but then the next launch finds no place to start in while this one ends: 148 x 32000 bf16 with 20 alternatives
+ * takes 7.6 us unsplit, 8.3 us in twos, 12 to 14 us in threes and fours; 100 x 131072 fp32 27, 19, and 18 us.  Shares of at most
+ * one batch of 128 threads run with 128. */
 template <typename T> static int lp_run(cudaStream_t st, LpParams &p, int n)
 {
     constexpr int V = LpType<T>::V;
-    while (p.split < 8 && (long long)n * p.split < 2 * 148 && p.len / (2 * p.split) >= 512 * V) p.split *= 2;
-    return p.len / p.split <= 128 * LP_U * V ? lp_launch<T, 128>(st, p, n) : lp_launch<T, 512>(st, p, n);
+    const int room = 2 * 148 / n, most = p.len / (LP_NT * V);
+    p.split = room < most ? room : most;
+    p.split = p.split < 1 ? 1 : p.split > LP_SPLIT ? LP_SPLIT : p.split;
+    return p.len / p.split <= 128 * LP_U * V ? lp_launch<T, 128>(st, p, n) : lp_launch<T, LP_NT>(st, p, n);
 }
 
 extern "C" int dRk_logprobs(dRk_stream stream, const void *logits, int type, long long ld, int n, int len, float scale, const int *labels, int m,
