@@ -8,6 +8,8 @@
 
 #define FP8_BLOCK 128                                   /* values under one scale, rows of a packed block, bytes of its rows */
 #define FP8_BLOCK_BYTES (FP8_BLOCK * FP8_BLOCK)
+#define FP8_MAX 448.0f
+#define FP8_FLOOR 0x1p-96f      /* smallest block maximum a scale is made from: 448 / A stays finite */
 
 static inline int fp8_blocks(int n) { return (int)(((long long)n + FP8_BLOCK - 1) / FP8_BLOCK); }
 
@@ -20,6 +22,9 @@ template <> __device__ __forceinline__ __half fp8_store<__half>(float v) { retur
 __device__ __forceinline__ float fp8_act(float v, int act) { return act && v < 0.0f ? 0.0f : v; }
 
 struct Fp8Params {
+    const void *in;
+    size_t ldi;
+    int in_type, Nin, vec;              /* vec: rows of `in` start on 16-byte boundaries */
     const float *sx, *scales, *bias;    /* sx [n][kbp], scales [ob][kb] */
     void *out;
     size_t ldo;
@@ -32,6 +37,7 @@ struct Fp8Tensor {
     CUtensorMap mapW, mapX;
     int pairs, mtiles, ntiles;          /* k_fp8_pair: pairs of CTAs, tiles of 256 rows and of 256 outputs; pairs = 0: k_fp8_swap */
     int nt;                             /* rows per tile of k_fp8_swap */
+    int fuse;                           /* 1: k_fp8_swap rounds the input itself, no launch in front */
     int split;                          /* CTAs of a cluster that share a tile's K blocks */
 };
 

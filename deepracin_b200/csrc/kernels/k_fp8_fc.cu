@@ -15,8 +15,6 @@
 #include <stdlib.h>
 #include "k_fp8.cuh"
 
-#define FP8_MAX 448.0f
-#define FP8_FLOOR 0x1p-96f      /* smallest block maximum a scale is made from: 448 / A stays finite */
 
 template <typename T> __device__ __forceinline__ float fp8_load(const T *p);
 template <> __device__ __forceinline__ float fp8_load(const float *p) { return *p; }
@@ -73,6 +71,10 @@ __global__ void __launch_bounds__(256) k_fp8_quantize_rows(const T *__restrict__
 }
 
 /* ------------------------------------------------------------------ weights
+ * The layer's kernel reads packed weights by TMA before it waits for the launch in front, so what writes them ends with this. */
+__device__ __forceinline__ void fp8_publish() { asm volatile("fence.proxy.async;\n\tfence.acq_rel.gpu;" ::: "memory"); }
+
+/*
  * One CTA per 128 x 128 block of w [Nin][Nout]: the block goes through shared memory, once for its largest magnitude and
  * once transposed into codes. */
 __global__ void __launch_bounds__(256) k_fp8_pack_weights(const float *__restrict__ w, unsigned char *__restrict__ codes, float *__restrict__ scales,
@@ -106,6 +108,7 @@ __global__ void __launch_bounds__(256) k_fp8_pack_weights(const float *__restric
         }
     }
     if (threadIdx.x == 0) scales[blockIdx.x] = __fdiv_rn(a, FP8_MAX);
+    fp8_publish();
 }
 
 __global__ void __launch_bounds__(256) k_fp8_pack_codes(const unsigned char *__restrict__ src, size_t ldw, const float *__restrict__ src_scales,
@@ -117,6 +120,7 @@ __global__ void __launch_bounds__(256) k_fp8_pack_codes(const unsigned char *__r
         codes[(size_t)blockIdx.x * FP8_BLOCK_BYTES + i] = o < Nout && k < Nin ? src[(size_t)o * ldw + k] : 0;
     }
     if (threadIdx.x == 0) scales[blockIdx.x] = src_scales[blockIdx.x];
+    fp8_publish();
 }
 
 __global__ void __launch_bounds__(256) k_fp8_unpack_weights(const unsigned char *__restrict__ codes, const float *__restrict__ scales, float *__restrict__ w,
@@ -133,10 +137,8 @@ __global__ void __launch_bounds__(256) k_fp8_unpack_weights(const unsigned char 
 
 /* ------------------------------------------------------------------ host side */
 struct dRk_Fp8FcPlan {
-    const void *in;
-    size_t ldi;
-    int in_type, Nin, dev, vec;
-    unsigned char *q;
+    int dev;
+    unsigned char *q;                   /* rounded input and its scales, in the caller's scratch */
     float *sx;
     Fp8Params p;
     Fp8Tensor t;
@@ -233,12 +235,12 @@ extern "C" dRk_Fp8FcPlan *dRk_fp8_fc_plan(const void *in, int in_type, long long
     if (cudaGetDevice(&dev) != cudaSuccess) { (void)cudaGetLastError(); fp8_refuse(who, "no CUDA device"); return NULL; }
     dRk_Fp8FcPlan *p = (dRk_Fp8FcPlan *)calloc(1, sizeof(*p));
     if (!p) { fp8_refuse(who, "out of host memory"); return NULL; }
-    p->in = in;
-    p->ldi = (size_t)ldi;
-    p->in_type = in_type;
-    p->Nin = Nin;
     p->dev = dev;
-    p->vec = (uintptr_t)in % 16 == 0 && (n == 1 || (size_t)ldi * isz % 16 == 0);
+    p->p.in = in;
+    p->p.ldi = (size_t)ldi;
+    p->p.in_type = in_type;
+    p->p.Nin = Nin;
+    p->p.vec = (uintptr_t)in % 16 == 0 && (n == 1 || (size_t)ldi * isz % 16 == 0);
     const int kb = fp8_blocks(Nin), ob = fp8_blocks(Nout);
     const unsigned char *codes = (const unsigned char *)packed;
     p->q = (unsigned char *)scratch;
@@ -264,7 +266,7 @@ extern "C" dRk_Fp8FcPlan *dRk_fp8_fc_plan(const void *in, int in_type, long long
 template <typename T> static int fp8_quantize(const dRk_Fp8FcPlan *p, cudaStream_t st)
 {
     const unsigned blocks = drk_blocks((size_t)p->p.n * p->p.kb, 16, 148u * 8u);
-    return drk_launched(drk_launch_dep(k_fp8_quantize_rows<T>, dim3(blocks), dim3(256), 0, st, (const T *)p->in, p->ldi, p->q, p->sx, p->p.n, p->Nin, p->p.kb, p->p.kbp, p->vec));
+    return drk_launched(drk_launch_dep(k_fp8_quantize_rows<T>, dim3(blocks), dim3(256), 0, st, (const T *)p->p.in, p->p.ldi, p->q, p->sx, p->p.n, p->p.Nin, p->p.kb, p->p.kbp, p->p.vec));
 }
 
 extern "C" int dRk_fp8_fc_run(dRk_stream stream, dRk_Fp8FcPlan *p)
@@ -273,8 +275,10 @@ extern "C" int dRk_fp8_fc_run(dRk_stream stream, dRk_Fp8FcPlan *p)
     const int dev = drk_stream_device("dRk_fp8_fc_run", stream, p->dev);
     if (dev < 0) return dev;
     cudaStream_t st = drk_stream(stream);
-    const int rc = p->in_type == DRK_F32 ? fp8_quantize<float>(p, st) : p->in_type == DRK_BF16 ? fp8_quantize<__nv_bfloat16>(p, st) : fp8_quantize<__half>(p, st);
-    if (rc) return rc;
+    if (!p->t.fuse) {
+        const int type = p->p.in_type, rc = type == DRK_F32 ? fp8_quantize<float>(p, st) : type == DRK_BF16 ? fp8_quantize<__nv_bfloat16>(p, st) : fp8_quantize<__half>(p, st);
+        if (rc) return rc;
+    }
     return drk_fp8_tensor_launch(st, &p->t, &p->p);
 }
 

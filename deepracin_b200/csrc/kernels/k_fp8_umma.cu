@@ -17,18 +17,30 @@ __device__ __forceinline__ void umma_f8(uint32_t tmem_d, uint64_t adesc, uint64_
 /* instruction descriptor: D = F32, A = B = e4m3, both K-major, M = m, N = n */
 __host__ __device__ constexpr uint32_t make_idesc_f8(int m, int n) { return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24); }
 
-__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16])
+/* One statement loads and waits: with a wait of its own that names the registers as its operands, the compiler copied them, and
+ * k_fp8_pair's additions took three times as long. */
+__device__ __forceinline__ void tmem_ld_wait(uint32_t taddr, uint32_t (&r)[16])
 {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 "
-                 "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+                 "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n\t"
+                 "tcgen05.wait::ld.sync.aligned;"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
                    "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
                  : "r"(taddr) : "memory");
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
-/* One statement loads and waits: with a wait of its own that names the registers as its operands, the compiler copied them, and
- * k_fp8_pair's additions took three times as long. */
-__device__ __forceinline__ void tmem_ld64(uint32_t taddr, uint32_t (&r)[64])
+__device__ __forceinline__ void tmem_ld_wait(uint32_t taddr, uint32_t (&r)[32])
+{
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+                 "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+                 "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n\t"
+                 "tcgen05.wait::ld.sync.aligned;"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+                   "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+                   "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+                   "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+                 : "r"(taddr) : "memory");
+}
+__device__ __forceinline__ void tmem_ld_wait(uint32_t taddr, uint32_t (&r)[64])
 {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x64.b32 "
                  "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
@@ -45,11 +57,6 @@ __device__ __forceinline__ void tmem_ld64(uint32_t taddr, uint32_t (&r)[64])
                    "=r"(r[48]), "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]),
                    "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63])
                  : "r"(taddr) : "memory");
-}
-/* two FP32 FMAs in one instruction */
-__device__ __forceinline__ void ffma2(unsigned long long &acc, unsigned long long a, uint32_t b0, uint32_t b1)
-{
-    asm("{\n\t.reg .b64 b;\n\tmov.b64 b, {%2, %3};\n\tfma.rn.f32x2 %0, %1, b, %0;\n\t}" : "+l"(acc) : "l"(a), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ bool elect_one()
 {
@@ -86,204 +93,6 @@ __device__ __forceinline__ void fp8_put(const Fp8Params &p, size_t r, int o, flo
     else static_cast<__half *>(p.out)[at] = fp8_store<__half>(v);
 }
 
-/*
- * Few rows: the weights are on the M side (a packed block of 128 outputs x 128 inputs per stage, the only large operand), NT
- * rows of the input on the N side.  A cluster of `split` CTAs shares the K blocks of one tile and adds its sums through
- * distributed shared memory, in the order of the ranks.  Warp 0 issues TMA, warp 1 the MMAs, warps 2-5 own the 128 outputs (one
- * per lane) and hold NT running sums each; block i's accumulator is one of SLOTS in TMEM.
- */
-template <int NT> struct SwapCfg {
-    static constexpr int B_BYTES = NT * FP8_BLOCK;
-    static constexpr int STAGE_BYTES = FP8_BLOCK_BYTES + B_BYTES;
-    static constexpr int STAGES = NT == 16 ? 6 : NT == 32 ? 5 : NT == 64 ? 4 : 6;
-    static constexpr int SLOTS = NT <= 64 ? 4 : 2;
-    static constexpr int TMEM_COLS = SLOTS * NT < 32 ? 32 : SLOTS * NT;
-    static constexpr int CTAS = NT <= 64 ? 2 : 1;               /* resident per SM */
-    static constexpr int SMEM = 1024 + STAGES * STAGE_BYTES + 4 * 2 * NT * 4 + 256;
-};
-
-template <int NT>
-__global__ void __launch_bounds__(192, SwapCfg<NT>::CTAS)
-k_fp8_swap(const __grid_constant__ CUtensorMap mapW, const __grid_constant__ CUtensorMap mapX, const Fp8Params p, int split)
-{
-    using C = SwapCfg<NT>;
-    extern __shared__ char smem_raw[];
-    const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
-    char *gen = smem_raw + (base - smem_u32(smem_raw));
-    float *factors = reinterpret_cast<float *>(gen + C::STAGES * C::STAGE_BYTES);       /* [4 warps][2][NT] */
-    char *tail = reinterpret_cast<char *>(factors + 4 * 2 * NT);
-    const uint32_t bars = smem_u32(tail);
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(tail + 8 * (2 * C::STAGES + 2 * C::SLOTS + 1));
-    volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
-    auto full_bar = [&](int s) { return bars + 8u * s; };
-    auto empty_bar = [&](int s) { return bars + 8u * (C::STAGES + s); };
-    auto tfull_bar = [&](int a) { return bars + 8u * (2 * C::STAGES + a); };
-    auto tempty_bar = [&](int a) { return bars + 8u * (2 * C::STAGES + C::SLOTS + a); };
-    const uint32_t drain_bar = bars + 8u * (2 * C::STAGES + 2 * C::SLOTS);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-
-    if (threadIdx.x == 0) {
-        for (int s = 0; s < C::STAGES; s++) { mbar_init(full_bar(s), 1); mbar_init(empty_bar(s), 1); }
-        for (int a = 0; a < C::SLOTS; a++) { mbar_init(tfull_bar(a), 1); mbar_init(tempty_bar(a), 4); }
-        mbar_init(drain_bar, 1);
-        *abort_flag = 0;
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    }
-    if (warp == 1) tmem_alloc(smem_u32(tmem_slot), C::TMEM_COLS);
-    tc_fence_before();
-    __syncthreads();
-    tc_fence_after();
-    const uint32_t tmem_base = *tmem_slot;
-
-    const int tile = blockIdx.x / split, rank = blockIdx.x - tile * split;
-    const int ot = tile % p.ob, r0 = (tile / p.ob) * NT;
-    const int b0 = (int)((long long)p.kb * rank / split), b1 = (int)((long long)p.kb * (rank + 1) / split);
-    unsigned long long acc[NT / 2];
-#pragma unroll
-    for (int j = 0; j < NT / 2; j++) acc[j] = 0ull;
-
-    if (warp == 0) {
-        if (lane == 0) {
-            int pre = 0;
-            /* weights do not depend on the launch in front (the rounding of the input): the first blocks are on their way before it ends */
-            for (; pre < C::STAGES && b0 + pre < b1; pre++) {
-                mbar_expect_tx(full_bar(pre), C::STAGE_BYTES);
-                tma_load_2d(base + pre * C::STAGE_BYTES, &mapW, 0, (ot * p.kb + b0 + pre) * FP8_BLOCK, full_bar(pre));
-            }
-            drk_dep_wait();
-            int stage = 0, issued = 0;
-            uint32_t phase = 0;
-            bool ok = true;
-            for (int b = b0; b < b1; b++) {
-                const uint32_t sw = base + stage * C::STAGE_BYTES;
-                if (issued >= pre) {
-                    if (!mbar_wait(empty_bar(stage), phase ^ 1u, abort_flag, p.status, 31)) { ok = false; break; }
-                    mbar_expect_tx(full_bar(stage), C::STAGE_BYTES);
-                    tma_load_2d(sw, &mapW, 0, (ot * p.kb + b) * FP8_BLOCK, full_bar(stage));
-                }
-                tma_load_2d(sw + FP8_BLOCK_BYTES, &mapX, 0, b * p.n + r0, full_bar(stage));
-                issued++;
-                if (++stage == C::STAGES) { stage = 0; phase ^= 1u; }
-            }
-            if (!ok) {      /* no copy may land after the exit */
-                const int pending = issued < C::STAGES ? issued : C::STAGES;
-                for (int i = 0; i < pending; i++) {
-                    if (--stage < 0) { stage = C::STAGES - 1; phase ^= 1u; }
-                    const long long t0 = clock64();
-                    while (!mbar_try(full_bar(stage), phase) && clock64() - t0 < WAIT_CYCLES) { }
-                }
-            }
-        }
-    } else if (warp == 1) {
-        if (lane == 0) {
-            constexpr uint32_t idesc = make_idesc_f8(128, NT);
-            int stage = 0, slot = 0;
-            uint32_t phase = 0, sphase = 0;
-            bool ok = true;
-            for (int b = b0; b < b1; b++) {
-                if (!mbar_wait(tempty_bar(slot), sphase ^ 1u, abort_flag, p.status, 32) ||
-                    !mbar_wait(full_bar(stage), phase, abort_flag, p.status, 33)) { ok = false; break; }
-                tc_fence_after();
-                const uint32_t sw = base + stage * C::STAGE_BYTES;
-                const uint64_t adesc = make_smem_desc(sw), bdesc = make_smem_desc(sw + FP8_BLOCK_BYTES);
-#pragma unroll
-                for (int j = 0; j < 4; j++)     /* 32 inputs each, 32 bytes further inside the swizzled row */
-                    umma_f8(tmem_base + (uint32_t)(slot * NT), adesc + (uint64_t)(j * 2), bdesc + (uint64_t)(j * 2), idesc, j ? 1u : 0u);
-                umma_commit(empty_bar(stage));
-                umma_commit(tfull_bar(slot));
-                if (++stage == C::STAGES) { stage = 0; phase ^= 1u; }
-                if (++slot == C::SLOTS) { slot = 0; sphase ^= 1u; }
-            }
-            if (!ok) umma_drain(drain_bar);
-        }
-    } else {
-        const int quarter = warp & 3;
-        float *mine = factors + quarter * 2 * NT;
-        constexpr int PER = (NT + 31) / 32;
-        float4 now[PER], next[PER];     /* sx of this lane's rows for the blocks of a group of four, and for the next group */
-        float sw, sw_next;
-        drk_dep_wait();     /* sx is written by the launch in front */
-        auto fetch = [&](int b) {
-#pragma unroll
-            for (int j = 0; j < PER; j++) {
-                const int r = j * 32 + lane;
-                next[j] = r < NT && r0 + r < p.n ? __ldcg(reinterpret_cast<const float4 *>(p.sx + (size_t)(r0 + r) * p.kbp + (b & ~3))) : make_float4(0.f, 0.f, 0.f, 0.f);
-            }
-        };
-        const float *swp = p.scales + (size_t)ot * p.kb;
-        if (b0 < b1) { fetch(b0); sw_next = __ldg(swp + b0); }
-        int slot = 0, flip = 0;
-        uint32_t sphase = 0;
-        for (int b = b0; b < b1; b++) {
-            float *f = mine + flip * NT;
-            if (b == b0 || (b & 3) == 0) {
-#pragma unroll
-                for (int j = 0; j < PER; j++) now[j] = next[j];
-                if ((b | 3) + 1 < b1) fetch((b | 3) + 1);
-            }
-            sw = sw_next;
-            if (b + 1 < b1) sw_next = __ldg(swp + b + 1);
-#pragma unroll
-            for (int j = 0; j < PER; j++)
-                if (j * 32 + lane < NT) f[j * 32 + lane] = ((b & 2) ? ((b & 1) ? now[j].w : now[j].z) : ((b & 1) ? now[j].y : now[j].x)) * sw;
-            __syncwarp();
-            if (!mbar_wait_warp(tfull_bar(slot), sphase, abort_flag, p.status, 34)) break;
-            tc_fence_after();
-            const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(slot * NT);
-#pragma unroll
-            for (int c0 = 0; c0 < NT; c0 += 16) {
-                uint32_t r[16];
-                tmem_ld16(taddr + (uint32_t)c0, r);
-#pragma unroll
-                for (int j = 0; j < 16; j += 4) {
-                    const ulonglong2 g = *reinterpret_cast<const ulonglong2 *>(f + c0 + j);
-                    ffma2(acc[(c0 + j) / 2], g.x, r[j], r[j + 1]);
-                    ffma2(acc[(c0 + j) / 2 + 1], g.y, r[j + 2], r[j + 3]);
-                }
-            }
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(tempty_bar(slot));
-            flip ^= 1;
-            if (++slot == C::SLOTS) { slot = 0; sphase ^= 1u; }
-        }
-    }
-    drk_dep_trigger();
-
-    /* every role is done: the stages hold the sums now, [NT rows][128 outputs] */
-    tc_fence_before();
-    __syncthreads();
-    if (warp == 1) tmem_dealloc(tmem_base, C::TMEM_COLS);
-    float *part = reinterpret_cast<float *>(gen);
-    const int ol = (warp & 3) * 32 + lane, o = ot * FP8_BLOCK + ol;
-    if (split == 1) {
-        if (warp >= 2 && o < p.Nout) {
-            const float bias = p.bias ? __ldg(p.bias + o) : 0.0f;
-#pragma unroll
-            for (int j = 0; j < NT; j++) {
-                const float v = __uint_as_float((uint32_t)(j & 1 ? acc[j / 2] >> 32 : acc[j / 2]));
-                if (r0 + j < p.n) fp8_put(p, (size_t)r0 + j, o, v + bias);
-            }
-        }
-        return;
-    }
-    if (warp >= 2)
-#pragma unroll
-        for (int j = 0; j < NT; j++)
-            if (r0 + j < p.n) part[j * FP8_BLOCK + ol] = __uint_as_float((uint32_t)(j & 1 ? acc[j / 2] >> 32 : acc[j / 2]));
-    cluster_sync();
-    if (warp >= 2) {
-        const float bias = p.bias && o < p.Nout ? __ldg(p.bias + o) : 0.0f;
-        for (int j = rank; j < NT && r0 + j < p.n; j += split) {
-            const uint32_t at = smem_u32(part + j * FP8_BLOCK + ol);
-            float v = 0.0f;
-            for (int s = 0; s < split; s++) v += ld_cluster(at, (uint32_t)s);
-            if (o < p.Nout) fp8_put(p, (size_t)r0 + j, o, v + bias);
-        }
-    }
-    cluster_sync();     /* the other CTAs read this one's sums until here */
-}
-
 /* a wait of a whole warp that holds many registers: no call inside, which would have them saved around it */
 __device__ __forceinline__ bool mbar_wait_warp_inline(uint32_t bar, uint32_t parity, volatile int *abort_flag, int *status, int code)
 {
@@ -312,6 +121,284 @@ __device__ __forceinline__ bool mbar_wait1(uint32_t bar, uint32_t parity, volati
     }
     return true;
 }
+/*
+ * Few rows: the weights are on the M side (a packed block of 128 outputs x 128 inputs per stage, the only large operand), NT
+ * rows of the input on the N side.  A cluster of `split` CTAs shares the K blocks of one tile and adds its sums through
+ * distributed shared memory, in the order of the ranks.  Warp 0 issues TMA, warp 1 the MMAs; four warps (eight from NT = 64 on)
+ * own the 128 outputs, one per lane, and add block after block times sx * sw to NT (NT / 2) sums each; a block's accumulator is
+ * one of SLOTS in TMEM.  The weights do not depend on the launch in front: their first blocks are on the way before it ends.
+ *
+ * FUSE (at most FUSE_ROWS rows): four more warps round the input themselves, a block each in turn, straight into the swizzled
+ * operand tile; what took two launches takes one.
+ */
+#define FUSE_ROWS 8
+template <int NT, bool FUSE> struct SwapCfg {
+    static constexpr int B_BYTES = NT * FP8_BLOCK;
+    static constexpr int STAGE_BYTES = FP8_BLOCK_BYTES + B_BYTES;
+    static constexpr int STAGES = NT == 16 ? 6 : NT == 32 ? 5 : NT == 64 ? 4 : 6;
+    static constexpr int SLOTS = NT <= 64 ? 4 : 2;
+    static constexpr int TMEM_COLS = SLOTS * NT < 32 ? 32 : SLOTS * NT;
+    static constexpr int CTAS = NT <= 64 ? 2 : 1;               /* resident per SM */
+    static constexpr int SUM_WARPS = NT <= 32 ? 4 : 8, COLS = NT * 4 / SUM_WARPS;       /* COLS: sums per lane */
+    static constexpr int THREADS = 32 * (2 + SUM_WARPS + (FUSE ? 4 : 0));
+    /* factors: a pair of slots per summing warp, or, written by the rounding warps, one per block that is under way: a stage is
+       filled again when its MMAs are done, and those wait for the accumulator of SLOTS blocks before */
+    static constexpr int RING = STAGES + SLOTS, FACTORS = FUSE ? RING * NT : SUM_WARPS * 2 * COLS;
+    static constexpr int SMEM = 1024 + STAGES * STAGE_BYTES + FACTORS * 4 + 256;
+};
+
+/* four values of a row from k on, zero behind Nin */
+__device__ __forceinline__ float4 fp8_load4(const Fp8Params &p, int r, int k)
+{
+    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    const size_t at = (size_t)r * p.ldi + k;
+    if (p.vec && k + 4 <= p.Nin) {
+        if (p.in_type == DRK_F32) return __ldg(reinterpret_cast<const float4 *>(static_cast<const float *>(p.in) + at));
+        const uint2 w = __ldg(reinterpret_cast<const uint2 *>(static_cast<const char *>(p.in) + 2 * at));
+        if (p.in_type == DRK_BF16)
+            return make_float4(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u), __uint_as_float(w.y << 16), __uint_as_float(w.y & 0xffff0000u));
+        const float2 a = __half22float2(*reinterpret_cast<const __half2 *>(&w.x)), b = __half22float2(*reinterpret_cast<const __half2 *>(&w.y));
+        return make_float4(a.x, a.y, b.x, b.y);
+    }
+    float *e = &v.x;
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+        if (k + j < p.Nin)
+            e[j] = p.in_type == DRK_F32    ? static_cast<const float *>(p.in)[at + j]
+                   : p.in_type == DRK_BF16 ? __bfloat162float(static_cast<const __nv_bfloat16 *>(p.in)[at + j])
+                                           : __half2float(static_cast<const __half *>(p.in)[at + j]);
+    return v;
+}
+
+template <int NT, bool FUSE>
+__global__ void __launch_bounds__((SwapCfg<NT, FUSE>::THREADS), (SwapCfg<NT, FUSE>::CTAS))
+k_fp8_swap(const __grid_constant__ CUtensorMap mapW, const __grid_constant__ CUtensorMap mapX, const __grid_constant__ Fp8Params p, int split)
+{
+    using C = SwapCfg<NT, FUSE>;
+    extern __shared__ char smem_raw[];
+    const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    char *gen = smem_raw + (base - smem_u32(smem_raw));
+    float *factors = reinterpret_cast<float *>(gen + C::STAGES * C::STAGE_BYTES);
+    char *tail = reinterpret_cast<char *>(factors + C::FACTORS);
+    const uint32_t bars = smem_u32(tail);
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(tail + 8 * (2 * C::STAGES + 2 * C::SLOTS + 1));
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
+    auto full_bar = [&](int s) { return bars + 8u * s; };
+    auto empty_bar = [&](int s) { return bars + 8u * (C::STAGES + s); };
+    auto tfull_bar = [&](int a) { return bars + 8u * (2 * C::STAGES + a); };
+    auto tempty_bar = [&](int a) { return bars + 8u * (2 * C::STAGES + C::SLOTS + a); };
+    const uint32_t drain_bar = bars + 8u * (2 * C::STAGES + 2 * C::SLOTS);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < C::STAGES; s++) { mbar_init(full_bar(s), FUSE ? 2 : 1); mbar_init(empty_bar(s), 1); }
+        for (int a = 0; a < C::SLOTS; a++) { mbar_init(tfull_bar(a), 1); mbar_init(tempty_bar(a), C::SUM_WARPS); }
+        mbar_init(drain_bar, 1);
+        *abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) tmem_alloc(smem_u32(tmem_slot), C::TMEM_COLS);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+
+    const int tile = blockIdx.x / split, rank = blockIdx.x - tile * split;
+    const int ot = tile % p.ob, r0 = (tile / p.ob) * NT;
+    const int b0 = (int)((long long)p.kb * rank / split), b1 = (int)((long long)p.kb * (rank + 1) / split);
+    constexpr uint32_t TX = FUSE ? FP8_BLOCK_BYTES : C::STAGE_BYTES;
+    float acc[C::COLS];
+#pragma unroll
+    for (int j = 0; j < C::COLS; j++) acc[j] = 0.0f;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            int pre = 0;
+            for (; pre < C::STAGES && b0 + pre < b1; pre++) {
+                mbar_expect_tx(full_bar(pre), TX);
+                tma_load_2d(base + pre * C::STAGE_BYTES, &mapW, 0, (ot * p.kb + b0 + pre) * FP8_BLOCK, full_bar(pre));
+            }
+            drk_dep_wait();
+            int stage = 0, issued = 0;
+            uint32_t phase = 0;
+            bool ok = true;
+            for (int b = b0; b < b1; b++) {
+                const uint32_t sw = base + stage * C::STAGE_BYTES;
+                if (issued >= pre) {
+                    if (!mbar_wait1(empty_bar(stage), phase ^ 1u, abort_flag, p.status, 31)) { ok = false; break; }
+                    mbar_expect_tx(full_bar(stage), TX);
+                    tma_load_2d(sw, &mapW, 0, (ot * p.kb + b) * FP8_BLOCK, full_bar(stage));
+                }
+                if (!FUSE) tma_load_2d(sw + FP8_BLOCK_BYTES, &mapX, 0, b * p.n + r0, full_bar(stage));
+                issued++;
+                if (++stage == C::STAGES) { stage = 0; phase ^= 1u; }
+            }
+            if (!ok) {      /* no copy may land after the exit */
+                const int pending = issued < C::STAGES ? issued : C::STAGES;
+                for (int i = 0; i < pending; i++) {
+                    if (--stage < 0) { stage = C::STAGES - 1; phase ^= 1u; }
+                    const long long t0 = clock64();
+                    while (!mbar_try(full_bar(stage), phase) && clock64() - t0 < WAIT_CYCLES) { }
+                }
+            }
+        }
+    } else if (warp == 1) {
+        constexpr uint32_t idesc = make_idesc_f8(128, NT);
+        int stage = 0, slot = 0;
+        uint32_t phase = 0, sphase = 0;
+        bool ok = true;
+        for (int b = b0; b < b1; b++) {
+            const bool full = mbar_try(full_bar(stage), phase), room = mbar_try(tempty_bar(slot), sphase ^ 1u);
+            if (!__all_sync(0xffffffffu, full && room) &&
+                (!mbar_wait_warp_inline(full_bar(stage), phase, abort_flag, p.status, 33) ||
+                 !mbar_wait_warp_inline(tempty_bar(slot), sphase ^ 1u, abort_flag, p.status, 32))) { ok = false; break; }
+            tc_fence_after();
+            if (elect_one()) {
+                const uint32_t sw = base + stage * C::STAGE_BYTES;
+                const uint64_t adesc = make_smem_desc(sw), bdesc = make_smem_desc(sw + FP8_BLOCK_BYTES);
+#pragma unroll
+                for (int j = 0; j < 4; j++)     /* 32 inputs each, 32 bytes further inside the swizzled row */
+                    umma_f8(tmem_base + (uint32_t)(slot * NT), adesc + (uint64_t)(j * 2), bdesc + (uint64_t)(j * 2), idesc, j ? 1u : 0u);
+                umma_commit(empty_bar(stage));
+                umma_commit(tfull_bar(slot));
+            }
+            __syncwarp();
+            if (++stage == C::STAGES) { stage = 0; phase ^= 1u; }
+            if (++slot == C::SLOTS) { slot = 0; sphase ^= 1u; }
+        }
+        if (!ok && elect_one()) umma_drain(drain_bar);
+        __syncwarp();
+    } else if (warp < 2 + C::SUM_WARPS) {
+        const int quarter = warp & 3, part = (warp - 2) >> 2, c0 = part * C::COLS;
+        float *mine = factors + (warp - 2) * 2 * C::COLS;
+        constexpr int PER = (C::COLS + 31) / 32;
+        float4 now[PER], next[PER];     /* sx of this lane's rows for the blocks of a group of four, and for the next group */
+        float sw = 0.0f, sw_next = 0.0f;
+        const float *swp = p.scales + (size_t)ot * p.kb;
+        drk_dep_wait();     /* sx is written by the launch in front; the rows in p.out may still be read by it */
+        auto fetch = [&](int b) {
+#pragma unroll
+            for (int j = 0; j < PER; j++) {
+                const int r = c0 + j * 32 + lane;
+                next[j] = j * 32 + lane < C::COLS && r0 + r < p.n ? __ldcg(reinterpret_cast<const float4 *>(p.sx + (size_t)(r0 + r) * p.kbp + (b & ~3)))
+                                                                  : make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+        };
+        if (!FUSE && b0 < b1) { fetch(b0); sw_next = __ldg(swp + b0); }
+        int slot = 0, flip = 0;
+        uint32_t sphase = 0;
+        for (int b = b0; b < b1; b++) {
+            const float *f = factors + ((b - b0) % C::RING) * NT + c0;
+            if (!FUSE) {
+                float *g = mine + flip * C::COLS;
+                if (b == b0 || (b & 3) == 0) {
+#pragma unroll
+                    for (int j = 0; j < PER; j++) now[j] = next[j];
+                    if ((b | 3) + 1 < b1) fetch((b | 3) + 1);
+                }
+                sw = sw_next;
+                if (b + 1 < b1) sw_next = __ldg(swp + b + 1);
+#pragma unroll
+                for (int j = 0; j < PER; j++)
+                    if (j * 32 + lane < C::COLS) g[j * 32 + lane] = ((b & 2) ? ((b & 1) ? now[j].w : now[j].z) : ((b & 1) ? now[j].y : now[j].x)) * sw;
+                __syncwarp();
+                f = g;
+                flip ^= 1;
+            }
+            if (!mbar_wait_warp_inline(tfull_bar(slot), sphase, abort_flag, p.status, 34)) break;
+            tc_fence_after();
+            const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(slot * NT + c0);
+            constexpr int STEP = C::COLS < 32 ? 16 : 32;
+#pragma unroll
+            for (int c = 0; c < C::COLS; c += STEP) {
+                uint32_t r[STEP];
+                tmem_ld_wait(taddr + (uint32_t)c, r);
+                if (c + STEP >= C::COLS) {      /* the accumulator is in registers */
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(tempty_bar(slot));
+                }
+#pragma unroll
+                for (int j = 0; j < STEP; j += 4) {
+                    const float4 g = *reinterpret_cast<const float4 *>(f + c + j);
+                    acc[c + j] = fmaf(g.x, __uint_as_float(r[j]), acc[c + j]);
+                    acc[c + j + 1] = fmaf(g.y, __uint_as_float(r[j + 1]), acc[c + j + 1]);
+                    acc[c + j + 2] = fmaf(g.z, __uint_as_float(r[j + 2]), acc[c + j + 2]);
+                    acc[c + j + 3] = fmaf(g.w, __uint_as_float(r[j + 3]), acc[c + j + 3]);
+                }
+            }
+            if (++slot == C::SLOTS) { slot = 0; sphase ^= 1u; }
+        }
+    } else if (FUSE) {
+        /* warp w rounds the blocks w, w + 4, ...: a row's 128 values are four per lane */
+        const float *swp = p.scales + (size_t)ot * p.kb;
+        float4 x[FUSE_ROWS];
+        float sw = 0.0f;
+        int b = b0 + warp - 2 - C::SUM_WARPS;
+        drk_dep_wait();
+        if (b < b1) {
+            sw = __ldg(swp + b);
+#pragma unroll
+            for (int r = 0; r < FUSE_ROWS; r++) if (r < p.n) x[r] = fp8_load4(p, r, b * FP8_BLOCK + lane * 4);
+        }
+        for (; b < b1; b += 4) {
+            const int i = b - b0, stage = i % C::STAGES;
+            const float s = sw;
+            if (b + 4 < b1) sw = __ldg(swp + b + 4);
+            if (i >= C::STAGES && !mbar_wait_warp_inline(empty_bar(stage), ((uint32_t)(i / C::STAGES) & 1u) ^ 1u, abort_flag, p.status, 35)) break;
+            char *tile_x = gen + stage * C::STAGE_BYTES + FP8_BLOCK_BYTES;
+            float *f = factors + (i % C::RING) * NT;
+#pragma unroll
+            for (int r = 0; r < FUSE_ROWS; r++) {
+                if (r >= p.n) break;
+                const float4 v = x[r];
+                if (b + 4 < b1) x[r] = fp8_load4(p, r, (b + 4) * FP8_BLOCK + lane * 4);
+                float a = fmaxf(fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))), FP8_FLOOR);
+                a = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(a)));      /* positive floats compare as whole numbers */
+                const float inv = __fdiv_rn(FP8_MAX, a);
+                const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(v.x * inv, v.y * inv), __NV_SATFINITE, __NV_E4M3);
+                const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(v.z * inv, v.w * inv), __NV_SATFINITE, __NV_E4M3);
+                *reinterpret_cast<uint32_t *>(tile_x + r * FP8_BLOCK + ((((lane >> 2) ^ (r & 7)) << 4) | ((lane & 3) << 2))) = lo | (hi << 16);
+                if (lane == 0) f[r] = __fdiv_rn(a, FP8_MAX) * s;
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(full_bar(stage));
+        }
+    }
+    drk_dep_trigger();
+
+    /* every role is done: the stages hold the sums now, [NT rows][128 outputs] */
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) tmem_dealloc(tmem_base, C::TMEM_COLS);
+    const bool summing = warp >= 2 && warp < 2 + C::SUM_WARPS;
+    const int ol = (warp & 3) * 32 + lane, o = ot * FP8_BLOCK + ol, part = (warp - 2) >> 2, c0 = part * C::COLS;
+    const float bias = summing && p.bias && o < p.Nout ? __ldg(p.bias + o) : 0.0f;
+    if (split == 1) {
+        if (summing && o < p.Nout)
+#pragma unroll
+            for (int j = 0; j < C::COLS; j++) if (r0 + c0 + j < p.n) fp8_put(p, (size_t)r0 + c0 + j, o, acc[j] + bias);
+        return;
+    }
+    float *sums = reinterpret_cast<float *>(gen);
+    if (summing)
+#pragma unroll
+        for (int j = 0; j < C::COLS; j++) if (r0 + c0 + j < p.n) sums[(c0 + j) * FP8_BLOCK + ol] = acc[j];
+    cluster_sync();
+    if (summing)
+        for (int j = rank + part * split; j < NT && r0 + j < p.n; j += split * (C::SUM_WARPS / 4)) {
+            const uint32_t at = smem_u32(sums + j * FP8_BLOCK + ol);
+            float v[8], sum = 0.0f;
+#pragma unroll
+            for (int s = 0; s < 8; s++) v[s] = s < split ? ld_cluster(at, (uint32_t)s) : 0.0f;
+#pragma unroll
+            for (int s = 0; s < 8; s++) sum += v[s];
+            if (o < p.Nout) fp8_put(p, (size_t)r0 + j, o, sum + bias);
+        }
+    cluster_sync();     /* the other CTAs read this one's sums until here */
+}
+
 /*
  * Many rows: a pair of CTAs (cta_group::2) computes 256 rows x 256 outputs, persistent over the tiles.  Per 128 inputs each CTA
  * fetches its 128 rows of the input and 64 rows of each of the tile's two weight blocks (32 KiB a stage; a single CTA's tile of
@@ -356,7 +443,7 @@ __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_bar)
 }
 
 __global__ void __launch_bounds__(384, 1)
-k_fp8_pair(const __grid_constant__ CUtensorMap mapW, const __grid_constant__ CUtensorMap mapX, const Fp8Params p, int mtiles, int ntiles)
+k_fp8_pair(const __grid_constant__ CUtensorMap mapW, const __grid_constant__ CUtensorMap mapX, const __grid_constant__ Fp8Params p, int mtiles, int ntiles)
 {
     using C = PairCfg;
     extern __shared__ char smem_raw[];
@@ -526,7 +613,7 @@ k_fp8_pair(const __grid_constant__ CUtensorMap mapW, const __grid_constant__ CUt
 #pragma unroll
                 for (int c = 0; c < 2; c++) {
                     uint32_t r[64];
-                    tmem_ld64(at + 64u * c, r);
+                    tmem_ld_wait(at + 64u * c, r);
                     if (c == 1) {
                         release(a);
                         const int b1 = b + 1;
@@ -626,13 +713,15 @@ int drk_fp8_tensor_plan(Fp8Tensor *t, const Fp8Params *p, const void *codes, con
     const int tiles = p->ob * ((p->n + t->nt - 1) / t->nt);
     t->split = 1;
     while (t->split < 8 && tiles * t->split < sms && t->split * 4 <= p->kb) t->split *= 2;
+    t->fuse = !t->pairs && p->n <= FUSE_ROWS;
     /* the attribute holds for the current device, which is the plan's */
     const cudaFuncAttribute dyn = cudaFuncAttributeMaxDynamicSharedMemorySize;
     const cudaError_t e = t->pairs      ? cudaFuncSetAttribute(k_fp8_pair, dyn, PairCfg::SMEM)
-                          : t->nt == 16 ? cudaFuncSetAttribute(k_fp8_swap<16>, dyn, SwapCfg<16>::SMEM)
-                          : t->nt == 32 ? cudaFuncSetAttribute(k_fp8_swap<32>, dyn, SwapCfg<32>::SMEM)
-                          : t->nt == 64 ? cudaFuncSetAttribute(k_fp8_swap<64>, dyn, SwapCfg<64>::SMEM)
-                                        : cudaFuncSetAttribute(k_fp8_swap<128>, dyn, SwapCfg<128>::SMEM);
+                          : t->fuse     ? cudaFuncSetAttribute(k_fp8_swap<16, true>, dyn, SwapCfg<16, true>::SMEM)
+                          : t->nt == 16 ? cudaFuncSetAttribute(k_fp8_swap<16, false>, dyn, SwapCfg<16, false>::SMEM)
+                          : t->nt == 32 ? cudaFuncSetAttribute(k_fp8_swap<32, false>, dyn, SwapCfg<32, false>::SMEM)
+                          : t->nt == 64 ? cudaFuncSetAttribute(k_fp8_swap<64, false>, dyn, SwapCfg<64, false>::SMEM)
+                                        : cudaFuncSetAttribute(k_fp8_swap<128, false>, dyn, SwapCfg<128, false>::SMEM);
     if (e != cudaSuccess) return -1;
     if (encode_rows(&t->mapW, codes, (size_t)p->ob * p->kb * FP8_BLOCK, t->pairs ? 64 : FP8_BLOCK)) return -1;
     return encode_rows(&t->mapX, q, (size_t)p->kb * p->n, t->nt);
@@ -657,13 +746,19 @@ static int cluster_launch(void (*kernel)(KArgs...), unsigned grid, unsigned bloc
     return drk_launched(cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...));
 }
 
-template <int NT> static int swap_launch(cudaStream_t st, const Fp8Tensor *t, const Fp8Params *p)
+template <int NT, bool FUSE> static int swap_launch(cudaStream_t st, const Fp8Tensor *t, const Fp8Params *p)
 {
-    return cluster_launch(k_fp8_swap<NT>, (unsigned)(p->ob * ((p->n + NT - 1) / NT) * t->split), 192, t->split, SwapCfg<NT>::SMEM, st, t->mapW, t->mapX, *p, t->split);
+    using C = SwapCfg<NT, FUSE>;
+    return cluster_launch(k_fp8_swap<NT, FUSE>, (unsigned)(p->ob * ((p->n + NT - 1) / NT) * t->split), C::THREADS, t->split, C::SMEM, st, t->mapW, t->mapX, *p,
+                          t->split);
 }
 
 int drk_fp8_tensor_launch(cudaStream_t st, const Fp8Tensor *t, const Fp8Params *p)
 {
     if (t->pairs) return cluster_launch(k_fp8_pair, 2u * t->pairs, 384, 2, PairCfg::SMEM, st, t->mapW, t->mapX, *p, t->mtiles, t->ntiles);
-    return t->nt == 16 ? swap_launch<16>(st, t, p) : t->nt == 32 ? swap_launch<32>(st, t, p) : t->nt == 64 ? swap_launch<64>(st, t, p) : swap_launch<128>(st, t, p);
+    if (t->fuse) return swap_launch<16, true>(st, t, p);
+    return t->nt == 16   ? swap_launch<16, false>(st, t, p)
+           : t->nt == 32 ? swap_launch<32, false>(st, t, p)
+           : t->nt == 64 ? swap_launch<64, false>(st, t, p)
+                         : swap_launch<128, false>(st, t, p);
 }
