@@ -38,6 +38,7 @@ struct Fp8Tensor {
     int pairs, mtiles, ntiles;          /* k_fp8_pair: pairs of CTAs, tiles of 256 rows and of 256 outputs; pairs = 0: k_fp8_swap */
     int nt;                             /* rows per tile of k_fp8_swap */
     int fuse;                           /* 1: k_fp8_swap rounds the input itself, no launch in front */
+    int stages;                         /* K blocks of the largest share: no more stages than that */
     int split;                          /* CTAs of a cluster that share a tile's K blocks */
 };
 

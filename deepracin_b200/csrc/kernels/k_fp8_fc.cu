@@ -23,49 +23,63 @@ template <> __device__ __forceinline__ float fp8_load(const __half *p) { return 
 __device__ __forceinline__ float fp8_decode(unsigned char c) { return __half2float(__half(__nv_cvt_fp8_to_halfraw(c, __NV_E4M3))); }
 
 /* ------------------------------------------------------------------ activations
- * A half warp owns a block of 128 values of one row: 8 per lane.  q: [block][n rows][128], sx: [n rows][kbp blocks]. */
-template <typename T>
+ * A half warp owns a block of 128 values of one row, 8 per lane, and asks for U blocks before it rounds the first: bound by HBM
+ * (reads sizeof(T), writes one byte a value).  4096 x 8192 bf16 with one block under way: 30 us; U = 4: QUANT_BIG.
+ * q: [block][n rows][128], sx: [n rows][kbp blocks]. */
+template <typename T, int U>
 __global__ void __launch_bounds__(256) k_fp8_quantize_rows(const T *__restrict__ in, size_t ldi, unsigned char *__restrict__ q, float *__restrict__ sx,
                                                            int n, int Nin, int kb, int kbp, int vec)
 {
     drk_dep_wait();
     drk_dep_trigger();
+    constexpr int W = sizeof(T) / 2;        /* 16-byte loads of 8 values */
     const int sub = threadIdx.x & 15;
-    const size_t total = (size_t)n * kb, step = (size_t)gridDim.x * (blockDim.x / 16);
+    const unsigned total = (unsigned)n * (unsigned)kb, halves = gridDim.x * (blockDim.x / 16);
     /* whole warps stay in the loop: both halves shuffle together */
-    for (size_t w0 = (size_t)blockIdx.x * (blockDim.x / 16) + (threadIdx.x >> 5) * 2; w0 < total; w0 += step) {
-        const size_t i = w0 + ((threadIdx.x >> 4) & 1);
-        const bool ok = i < total;
-        const size_t r = ok ? i / kb : 0;
-        const int b = ok ? (int)(i - r * kb) : 0, k0 = b * FP8_BLOCK + sub * 8;
-        const T *src = in + r * ldi + k0;
-        float v[8];
-        if (ok && vec && k0 + 8 <= Nin) {
-            uint4 raw[sizeof(T) / 2];
+    for (unsigned i0 = blockIdx.x * (blockDim.x / 16) + (threadIdx.x >> 5) * 2; i0 < total; i0 += U * halves) {
+        uint4 raw[U][W];
+        unsigned row[U], blk[U];
 #pragma unroll
-            for (int j = 0; j < (int)(sizeof(T) / 2); j++) raw[j] = __ldg(reinterpret_cast<const uint4 *>(src) + j);
+        for (int u = 0; u < U; u++) {
+            const unsigned i = i0 + ((threadIdx.x >> 4) & 1) + u * halves;
+            row[u] = i < total ? i / (unsigned)kb : 0xffffffffu;
+            blk[u] = i - row[u] * (unsigned)kb;
 #pragma unroll
-            for (int j = 0; j < 8; j++) v[j] = fp8_load(reinterpret_cast<const T *>(raw) + j);
-        } else {
+            for (int j = 0; j < W; j++) raw[u][j] = make_uint4(0u, 0u, 0u, 0u);
+            if (row[u] == 0xffffffffu) continue;
+            const int k0 = (int)blk[u] * FP8_BLOCK + sub * 8;
+            const T *src = in + row[u] * ldi + k0;
+            if (vec && k0 + 8 <= Nin) {
 #pragma unroll
-            for (int j = 0; j < 8; j++) v[j] = ok && k0 + j < Nin ? fp8_load(src + j) : 0.0f;
+                for (int j = 0; j < W; j++) raw[u][j] = __ldg(reinterpret_cast<const uint4 *>(src) + j);
+            } else {
+                T *one = reinterpret_cast<T *>(raw[u]);
+#pragma unroll
+                for (int j = 0; j < 8; j++) if (k0 + j < Nin) one[j] = src[j];
+            }
         }
-        float a = FP8_FLOOR;
 #pragma unroll
-        for (int j = 0; j < 8; j++) a = fmaxf(a, fabsf(v[j]));
+        for (int u = 0; u < U; u++) {
+            if (u > 0 && i0 + u * halves >= total) break;       /* the same for the whole warp: i0 is even, and so is halves */
+            float v[8], a = FP8_FLOOR;
 #pragma unroll
-        for (int o = 8; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o));
-        const float inv = __fdiv_rn(FP8_MAX, a);
-        uint32_t c[2];
+            for (int j = 0; j < 8; j++) v[j] = fp8_load(reinterpret_cast<const T *>(raw[u]) + j);
 #pragma unroll
-        for (int j = 0; j < 2; j++) {
-            const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(v[4 * j] * inv, v[4 * j + 1] * inv), __NV_SATFINITE, __NV_E4M3);
-            const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(v[4 * j + 2] * inv, v[4 * j + 3] * inv), __NV_SATFINITE, __NV_E4M3);
-            c[j] = lo | (hi << 16);
-        }
-        if (ok) {
-            *reinterpret_cast<uint2 *>(q + ((size_t)b * n + r) * FP8_BLOCK + sub * 8) = make_uint2(c[0], c[1]);
-            if (sub == 0) sx[r * kbp + b] = __fdiv_rn(a, FP8_MAX);
+            for (int j = 0; j < 8; j++) a = fmaxf(a, fabsf(v[j]));
+#pragma unroll
+            for (int o = 8; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o));
+            const float inv = __fdiv_rn(FP8_MAX, a);
+            uint32_t c[2];
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(v[4 * j] * inv, v[4 * j + 1] * inv), __NV_SATFINITE, __NV_E4M3);
+                const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(v[4 * j + 2] * inv, v[4 * j + 3] * inv), __NV_SATFINITE, __NV_E4M3);
+                c[j] = lo | (hi << 16);
+            }
+            if (row[u] != 0xffffffffu) {
+                *reinterpret_cast<uint2 *>(q + ((size_t)blk[u] * n + row[u]) * FP8_BLOCK + sub * 8) = make_uint2(c[0], c[1]);
+                if (sub == 0) sx[(size_t)row[u] * kbp + blk[u]] = __fdiv_rn(a, FP8_MAX);
+            }
         }
     }
 }
@@ -265,8 +279,12 @@ extern "C" dRk_Fp8FcPlan *dRk_fp8_fc_plan(const void *in, int in_type, long long
 
 template <typename T> static int fp8_quantize(const dRk_Fp8FcPlan *p, cudaStream_t st)
 {
-    const unsigned blocks = drk_blocks((size_t)p->p.n * p->p.kb, 16, 148u * 8u);
-    return drk_launched(drk_launch_dep(k_fp8_quantize_rows<T>, dim3(blocks), dim3(256), 0, st, (const T *)p->p.in, p->p.ldi, p->q, p->sx, p->p.n, p->p.Nin, p->p.kb, p->p.kbp, p->p.vec));
+    /* few blocks: one for each half warp; many: four under way in each */
+    const size_t halves = (size_t)p->p.n * p->p.kb;
+    const bool many = halves > 4 * 16 * 148 * 4;
+    const unsigned blocks = drk_blocks(many ? (halves + 3) / 4 : halves, 16, 148u * 16u);
+    return drk_launched(drk_launch_dep(many ? k_fp8_quantize_rows<T, 4> : k_fp8_quantize_rows<T, 1>, dim3(blocks), dim3(256), 0, st, (const T *)p->p.in,
+                                       p->p.ldi, p->q, p->sx, p->p.n, p->p.Nin, p->p.kb, p->p.kbp, p->p.vec));
 }
 
 extern "C" int dRk_fp8_fc_run(dRk_stream stream, dRk_Fp8FcPlan *p)

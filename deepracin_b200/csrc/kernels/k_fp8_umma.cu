@@ -78,11 +78,16 @@ __device__ __forceinline__ void cluster_sync()
     __syncwarp();
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-__device__ __forceinline__ float ld_cluster(uint32_t saddr, uint32_t rank)
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait()
 {
-    float v;
-    asm volatile("{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %1, %2;\n\tld.shared::cluster.f32 %0, [a];\n\t}" : "=f"(v) : "r"(saddr), "r"(rank) : "memory");
-    return v;
+    __syncwarp();
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+/* a store to this address in the shared memory of the cluster's CTA `rank` */
+__device__ __forceinline__ void st_cluster(uint32_t saddr, uint32_t rank, float v)
+{
+    asm volatile("{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %0, %1;\n\tst.shared::cluster.f32 [a], %2;\n\t}" ::"r"(saddr), "r"(rank), "f"(v) : "memory");
 }
 __device__ __forceinline__ void fp8_put(const Fp8Params &p, size_t r, int o, float v)
 {
@@ -123,28 +128,30 @@ __device__ __forceinline__ bool mbar_wait1(uint32_t bar, uint32_t parity, volati
 }
 /*
  * Few rows: the weights are on the M side (a packed block of 128 outputs x 128 inputs per stage, the only large operand), NT
- * rows of the input on the N side.  A cluster of `split` CTAs shares the K blocks of one tile and adds its sums through
- * distributed shared memory, in the order of the ranks.  Warp 0 issues TMA, warp 1 the MMAs; four warps (eight from NT = 64 on)
- * own the 128 outputs, one per lane, and add block after block times sx * sw to NT (NT / 2) sums each; a block's accumulator is
- * one of SLOTS in TMEM.  The weights do not depend on the launch in front: their first blocks are on the way before it ends.
+ * rows of the input on the N side.  A cluster of `split` CTAs shares the K blocks of one tile; each sends its sums of a row to
+ * the CTA that owns the row (distributed shared memory), which adds them in the order of the ranks.  Warp 0 issues TMA, warp 1 the MMAs; two groups of four warps own the
+ * 128 outputs, one per lane, and add the blocks times sx * sw to NT sums each, taking turns (what a block costs them beside the
+ * additions -- the wait, the factors -- is 350 of 600 clocks); with NT = 128 each has half of the rows instead.  A block's
+ * accumulator is one of SLOTS in TMEM.  The weights do not depend on the launch in front: their first blocks are on the way before it ends.
  *
  * FUSE (at most FUSE_ROWS rows): four more warps round the input themselves, a block each in turn, straight into the swizzled
  * operand tile; what took two launches takes one.
  */
-#define FUSE_ROWS 8
+#define FUSE_ROWS 4
 template <int NT, bool FUSE> struct SwapCfg {
     static constexpr int B_BYTES = NT * FP8_BLOCK;
     static constexpr int STAGE_BYTES = FP8_BLOCK_BYTES + B_BYTES;
-    static constexpr int STAGES = NT == 16 ? 6 : NT == 32 ? 5 : NT == 64 ? 4 : 6;
+    static constexpr int STAGES = NT == 16 ? 10 : NT == 32 ? 9 : NT == 64 ? 6 : 4;       /* at most: fewer for a short share */
     static constexpr int SLOTS = NT <= 64 ? 4 : 2;
-    static constexpr int TMEM_COLS = SLOTS * NT < 32 ? 32 : SLOTS * NT;
-    static constexpr int CTAS = NT <= 64 ? 2 : 1;               /* resident per SM */
-    static constexpr int SUM_WARPS = NT <= 32 ? 4 : 8, COLS = NT * 4 / SUM_WARPS;       /* COLS: sums per lane */
-    static constexpr int THREADS = 32 * (2 + SUM_WARPS + (FUSE ? 4 : 0));
+    static constexpr int TMEM_COLS = SLOTS * NT;
+    static constexpr int GROUPS = NT <= 64 ? 2 : 1;             /* of summing warps that take turns */
+    static constexpr int COLS = GROUPS == 2 ? NT : NT / 2;      /* sums per lane */
+    static constexpr int THREADS = 32 * (2 + 8 + (FUSE ? 4 : 0));
     /* factors: a pair of slots per summing warp, or, written by the rounding warps, one per block that is under way: a stage is
        filled again when its MMAs are done, and those wait for the accumulator of SLOTS blocks before */
-    static constexpr int RING = STAGES + SLOTS, FACTORS = FUSE ? RING * NT : SUM_WARPS * 2 * COLS;
-    static constexpr int SMEM = 1024 + STAGES * STAGE_BYTES + FACTORS * 4 + 256;
+    static constexpr int RING = STAGES + SLOTS, FACTORS = FUSE ? RING * NT : 8 * 2 * COLS;
+    static constexpr int INBOX = GROUPS * NT * FP8_BLOCK;       /* floats: sums of the rows this CTA owns, from every group of every CTA */
+    static constexpr int smem(int stages) { return 1024 + stages * STAGE_BYTES + INBOX * 4 + FACTORS * 4 + 256; }
 };
 
 /* four values of a row from k on, zero behind Nin */
@@ -171,14 +178,15 @@ __device__ __forceinline__ float4 fp8_load4(const Fp8Params &p, int r, int k)
 }
 
 template <int NT, bool FUSE>
-__global__ void __launch_bounds__((SwapCfg<NT, FUSE>::THREADS), (SwapCfg<NT, FUSE>::CTAS))
-k_fp8_swap(const __grid_constant__ CUtensorMap mapW, const __grid_constant__ CUtensorMap mapX, const __grid_constant__ Fp8Params p, int split)
+__global__ void __launch_bounds__((SwapCfg<NT, FUSE>::THREADS), 1)
+k_fp8_swap(const __grid_constant__ CUtensorMap mapW, const __grid_constant__ CUtensorMap mapX, const __grid_constant__ Fp8Params p, int split, int stages)
 {
     using C = SwapCfg<NT, FUSE>;
     extern __shared__ char smem_raw[];
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     char *gen = smem_raw + (base - smem_u32(smem_raw));
-    float *factors = reinterpret_cast<float *>(gen + C::STAGES * C::STAGE_BYTES);
+    float *inbox = reinterpret_cast<float *>(gen + stages * C::STAGE_BYTES);
+    float *factors = inbox + C::INBOX;
     char *tail = reinterpret_cast<char *>(factors + C::FACTORS);
     const uint32_t bars = smem_u32(tail);
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(tail + 8 * (2 * C::STAGES + 2 * C::SLOTS + 1));
@@ -190,34 +198,40 @@ k_fp8_swap(const __grid_constant__ CUtensorMap mapW, const __grid_constant__ CUt
     const uint32_t drain_bar = bars + 8u * (2 * C::STAGES + 2 * C::SLOTS);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
+    const int tile = blockIdx.x / split, rank = blockIdx.x - tile * split;
+    const int ot = tile % p.ob, r0 = (tile / p.ob) * NT;
+    const int b0 = (int)((long long)p.kb * rank / split), b1 = (int)((long long)p.kb * (rank + 1) / split);
+    constexpr uint32_t TX = FUSE ? FP8_BLOCK_BYTES : C::STAGE_BYTES;
+    if (split > 1) cluster_arrive();    /* waited for before the first store into another CTA: it runs by then */
+    int pre = 0;        /* blocks whose weights are on the way before the launch in front has ended */
+
     if (threadIdx.x == 0) {
         for (int s = 0; s < C::STAGES; s++) { mbar_init(full_bar(s), FUSE ? 2 : 1); mbar_init(empty_bar(s), 1); }
-        for (int a = 0; a < C::SLOTS; a++) { mbar_init(tfull_bar(a), 1); mbar_init(tempty_bar(a), C::SUM_WARPS); }
+        for (int a = 0; a < C::SLOTS; a++) { mbar_init(tfull_bar(a), 1); mbar_init(tempty_bar(a), 8 / C::GROUPS); }
         mbar_init(drain_bar, 1);
         *abort_flag = 0;
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.mbarrier_init.release.cluster;\n\tfence.proxy.async.shared::cta;" ::: "memory");
+        for (; pre < stages && b0 + pre < b1; pre++) {
+            mbar_expect_tx(full_bar(pre), TX);
+            tma_load_2d(base + pre * C::STAGE_BYTES, &mapW, 0, (ot * p.kb + b0 + pre) * FP8_BLOCK, full_bar(pre));
+        }
     }
-    if (warp == 1) tmem_alloc(smem_u32(tmem_slot), C::TMEM_COLS);
+    /* No TMEM before the launch in front has ended: its CTAs may still ask for theirs on this SM, and would wait for ours */
+    if (warp == 1) {
+        drk_dep_wait();
+        tmem_alloc(smem_u32(tmem_slot), C::TMEM_COLS);
+    }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
 
-    const int tile = blockIdx.x / split, rank = blockIdx.x - tile * split;
-    const int ot = tile % p.ob, r0 = (tile / p.ob) * NT;
-    const int b0 = (int)((long long)p.kb * rank / split), b1 = (int)((long long)p.kb * (rank + 1) / split);
-    constexpr uint32_t TX = FUSE ? FP8_BLOCK_BYTES : C::STAGE_BYTES;
     float acc[C::COLS];
 #pragma unroll
     for (int j = 0; j < C::COLS; j++) acc[j] = 0.0f;
 
     if (warp == 0) {
         if (lane == 0) {
-            int pre = 0;
-            for (; pre < C::STAGES && b0 + pre < b1; pre++) {
-                mbar_expect_tx(full_bar(pre), TX);
-                tma_load_2d(base + pre * C::STAGE_BYTES, &mapW, 0, (ot * p.kb + b0 + pre) * FP8_BLOCK, full_bar(pre));
-            }
             drk_dep_wait();
             int stage = 0, issued = 0;
             uint32_t phase = 0;
@@ -231,12 +245,12 @@ k_fp8_swap(const __grid_constant__ CUtensorMap mapW, const __grid_constant__ CUt
                 }
                 if (!FUSE) tma_load_2d(sw + FP8_BLOCK_BYTES, &mapX, 0, b * p.n + r0, full_bar(stage));
                 issued++;
-                if (++stage == C::STAGES) { stage = 0; phase ^= 1u; }
+                if (++stage == stages) { stage = 0; phase ^= 1u; }
             }
             if (!ok) {      /* no copy may land after the exit */
-                const int pending = issued < C::STAGES ? issued : C::STAGES;
+                const int pending = issued < stages ? issued : stages;
                 for (int i = 0; i < pending; i++) {
-                    if (--stage < 0) { stage = C::STAGES - 1; phase ^= 1u; }
+                    if (--stage < 0) { stage = stages - 1; phase ^= 1u; }
                     const long long t0 = clock64();
                     while (!mbar_try(full_bar(stage), phase) && clock64() - t0 < WAIT_CYCLES) { }
                 }
@@ -263,13 +277,13 @@ k_fp8_swap(const __grid_constant__ CUtensorMap mapW, const __grid_constant__ CUt
                 umma_commit(tfull_bar(slot));
             }
             __syncwarp();
-            if (++stage == C::STAGES) { stage = 0; phase ^= 1u; }
+            if (++stage == stages) { stage = 0; phase ^= 1u; }
             if (++slot == C::SLOTS) { slot = 0; sphase ^= 1u; }
         }
         if (!ok && elect_one()) umma_drain(drain_bar);
         __syncwarp();
-    } else if (warp < 2 + C::SUM_WARPS) {
-        const int quarter = warp & 3, part = (warp - 2) >> 2, c0 = part * C::COLS;
+    } else if (warp < 10) {
+        const int quarter = warp & 3, part = (warp - 2) >> 2, c0 = C::GROUPS == 2 ? 0 : part * C::COLS;
         float *mine = factors + (warp - 2) * 2 * C::COLS;
         constexpr int PER = (C::COLS + 31) / 32;
         float4 now[PER], next[PER];     /* sx of this lane's rows for the blocks of a group of four, and for the next group */
@@ -284,20 +298,21 @@ k_fp8_swap(const __grid_constant__ CUtensorMap mapW, const __grid_constant__ CUt
                                                                   : make_float4(0.f, 0.f, 0.f, 0.f);
             }
         };
-        if (!FUSE && b0 < b1) { fetch(b0); sw_next = __ldg(swp + b0); }
-        int slot = 0, flip = 0;
+        const int first = b0 + (C::GROUPS == 2 ? part : 0);         /* this group's first block */
+        if (!FUSE && first < b1) { fetch(first); sw_next = __ldg(swp + first); }
+        int slot = C::GROUPS == 2 ? part : 0, flip = 0;
         uint32_t sphase = 0;
-        for (int b = b0; b < b1; b++) {
+        for (int b = first; b < b1; b += C::GROUPS) {
             const float *f = factors + ((b - b0) % C::RING) * NT + c0;
             if (!FUSE) {
                 float *g = mine + flip * C::COLS;
-                if (b == b0 || (b & 3) == 0) {
+                if (b == first || (b & 3) < C::GROUPS) {
 #pragma unroll
                     for (int j = 0; j < PER; j++) now[j] = next[j];
                     if ((b | 3) + 1 < b1) fetch((b | 3) + 1);
                 }
                 sw = sw_next;
-                if (b + 1 < b1) sw_next = __ldg(swp + b + 1);
+                if (b + C::GROUPS < b1) sw_next = __ldg(swp + b + C::GROUPS);
 #pragma unroll
                 for (int j = 0; j < PER; j++)
                     if (j * 32 + lane < C::COLS) g[j * 32 + lane] = ((b & 2) ? ((b & 1) ? now[j].w : now[j].z) : ((b & 1) ? now[j].y : now[j].x)) * sw;
@@ -327,14 +342,15 @@ k_fp8_swap(const __grid_constant__ CUtensorMap mapW, const __grid_constant__ CUt
                     acc[c + j + 3] = fmaf(g.w, __uint_as_float(r[j + 3]), acc[c + j + 3]);
                 }
             }
-            if (++slot == C::SLOTS) { slot = 0; sphase ^= 1u; }
+            slot += C::GROUPS;
+            if (slot >= C::SLOTS) { slot -= C::SLOTS; sphase ^= 1u; }
         }
     } else if (FUSE) {
         /* warp w rounds the blocks w, w + 4, ...: a row's 128 values are four per lane */
         const float *swp = p.scales + (size_t)ot * p.kb;
         float4 x[FUSE_ROWS];
         float sw = 0.0f;
-        int b = b0 + warp - 2 - C::SUM_WARPS;
+        int b = b0 + warp - 10;
         drk_dep_wait();
         if (b < b1) {
             sw = __ldg(swp + b);
@@ -342,10 +358,10 @@ k_fp8_swap(const __grid_constant__ CUtensorMap mapW, const __grid_constant__ CUt
             for (int r = 0; r < FUSE_ROWS; r++) if (r < p.n) x[r] = fp8_load4(p, r, b * FP8_BLOCK + lane * 4);
         }
         for (; b < b1; b += 4) {
-            const int i = b - b0, stage = i % C::STAGES;
+            const int i = b - b0, stage = i % stages;
             const float s = sw;
             if (b + 4 < b1) sw = __ldg(swp + b + 4);
-            if (i >= C::STAGES && !mbar_wait_warp_inline(empty_bar(stage), ((uint32_t)(i / C::STAGES) & 1u) ^ 1u, abort_flag, p.status, 35)) break;
+            if (i >= stages && !mbar_wait_warp_inline(empty_bar(stage), ((uint32_t)(i / stages) & 1u) ^ 1u, abort_flag, p.status, 35)) break;
             char *tile_x = gen + stage * C::STAGE_BYTES + FP8_BLOCK_BYTES;
             float *f = factors + (i % C::RING) * NT;
 #pragma unroll
@@ -368,35 +384,35 @@ k_fp8_swap(const __grid_constant__ CUtensorMap mapW, const __grid_constant__ CUt
     }
     drk_dep_trigger();
 
-    /* every role is done: the stages hold the sums now, [NT rows][128 outputs] */
     tc_fence_before();
     __syncthreads();
-    if (warp == 1) tmem_dealloc(tmem_base, C::TMEM_COLS);
-    const bool summing = warp >= 2 && warp < 2 + C::SUM_WARPS;
-    const int ol = (warp & 3) * 32 + lane, o = ot * FP8_BLOCK + ol, part = (warp - 2) >> 2, c0 = part * C::COLS;
+    if (split > 1) cluster_wait();
+    /* row j of the tile belongs to CTA j % split, a power of two; inbox [source][row / split][128 outputs] */
+    const bool summing = warp >= 2 && warp < 10;
+    const int part = (warp - 2) >> 2, ol = (warp & 3) * 32 + lane, o = ot * FP8_BLOCK + ol;
+    const int c0 = C::GROUPS == 2 ? 0 : part * C::COLS, lg = 31 - __clz(split), own = NT >> lg, sources = C::GROUPS * split;
     const float bias = summing && p.bias && o < p.Nout ? __ldg(p.bias + o) : 0.0f;
-    if (split == 1) {
-        if (summing && o < p.Nout)
+    if (summing) {
+        const uint32_t to = smem_u32(inbox + (C::GROUPS * rank + (C::GROUPS == 2 ? part : 0)) * own * FP8_BLOCK + ol);
 #pragma unroll
-            for (int j = 0; j < C::COLS; j++) if (r0 + c0 + j < p.n) fp8_put(p, (size_t)r0 + c0 + j, o, acc[j] + bias);
-        return;
-    }
-    float *sums = reinterpret_cast<float *>(gen);
-    if (summing)
-#pragma unroll
-        for (int j = 0; j < C::COLS; j++) if (r0 + c0 + j < p.n) sums[(c0 + j) * FP8_BLOCK + ol] = acc[j];
-    cluster_sync();
-    if (summing)
-        for (int j = rank + part * split; j < NT && r0 + j < p.n; j += split * (C::SUM_WARPS / 4)) {
-            const uint32_t at = smem_u32(sums + j * FP8_BLOCK + ol);
-            float v[8], sum = 0.0f;
-#pragma unroll
-            for (int s = 0; s < 8; s++) v[s] = s < split ? ld_cluster(at, (uint32_t)s) : 0.0f;
-#pragma unroll
-            for (int s = 0; s < 8; s++) sum += v[s];
-            if (o < p.Nout) fp8_put(p, (size_t)r0 + j, o, sum + bias);
+        for (int j = 0; j < C::COLS; j++) {
+            const int r = c0 + j;
+            if (r0 + r >= p.n) break;
+            st_cluster(to + (uint32_t)(r >> lg) * (FP8_BLOCK * 4), (uint32_t)(r & (split - 1)), acc[j]);
         }
-    cluster_sync();     /* the other CTAs read this one's sums until here */
+    }
+    __syncwarp();
+    if (split > 1) cluster_arrive();
+    if (warp == 1) tmem_dealloc(tmem_base, C::TMEM_COLS);
+    if (split > 1) cluster_wait();
+    else __syncthreads();
+    if (summing && o < p.Nout)
+        for (int q = part; q < own && r0 + q * split + rank < p.n; q += 2) {
+            float sum = 0.0f;
+#pragma unroll 4
+            for (int s = 0; s < sources; s++) sum += inbox[(s * own + q) * FP8_BLOCK + ol];
+            fp8_put(p, (size_t)r0 + q * split + rank, o, sum + bias);
+        }
 }
 
 /*
@@ -470,7 +486,7 @@ k_fp8_pair(const __grid_constant__ CUtensorMap mapW, const __grid_constant__ CUt
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 1) {
+    if (warp == 1) {    /* shared memory leaves no room for another CTA with TMEM on this SM: nobody waits for this one's */
         asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
     }
@@ -489,6 +505,7 @@ k_fp8_pair(const __grid_constant__ CUtensorMap mapW, const __grid_constant__ CUt
         mt = g * C::GROUP + left - nt * rows;
     };
 
+    /* registers: 384 threads x 168 at launch = 128 x 56 + 256 x 224 */
     if (warp < 4) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
         if (warp == 0) {
@@ -710,18 +727,20 @@ int drk_fp8_tensor_plan(Fp8Tensor *t, const Fp8Params *p, const void *codes, con
         t->pairs = t->mtiles * t->ntiles < sms / 2 ? t->mtiles * t->ntiles : sms / 2;
     }
     t->nt = p->n <= 16 ? 16 : p->n <= 32 ? 32 : p->n <= 64 ? 64 : 128;
-    const int tiles = p->ob * ((p->n + t->nt - 1) / t->nt);
+    /* as many shares of a tile's blocks as still run at once, one on an SM */
+    const int tiles = p->ob * ((p->n + t->nt - 1) / t->nt), room = sms;
     t->split = 1;
-    while (t->split < 8 && tiles * t->split < sms && t->split * 4 <= p->kb) t->split *= 2;
+    while (t->split < 8 && tiles * t->split * 2 <= room && t->split * 4 <= p->kb) t->split *= 2;
+    t->stages = (p->kb + t->split - 1) / t->split;
     t->fuse = !t->pairs && p->n <= FUSE_ROWS;
     /* the attribute holds for the current device, which is the plan's */
     const cudaFuncAttribute dyn = cudaFuncAttributeMaxDynamicSharedMemorySize;
     const cudaError_t e = t->pairs      ? cudaFuncSetAttribute(k_fp8_pair, dyn, PairCfg::SMEM)
-                          : t->fuse     ? cudaFuncSetAttribute(k_fp8_swap<16, true>, dyn, SwapCfg<16, true>::SMEM)
-                          : t->nt == 16 ? cudaFuncSetAttribute(k_fp8_swap<16, false>, dyn, SwapCfg<16, false>::SMEM)
-                          : t->nt == 32 ? cudaFuncSetAttribute(k_fp8_swap<32, false>, dyn, SwapCfg<32, false>::SMEM)
-                          : t->nt == 64 ? cudaFuncSetAttribute(k_fp8_swap<64, false>, dyn, SwapCfg<64, false>::SMEM)
-                                        : cudaFuncSetAttribute(k_fp8_swap<128, false>, dyn, SwapCfg<128, false>::SMEM);
+                          : t->fuse     ? cudaFuncSetAttribute(k_fp8_swap<16, true>, dyn, SwapCfg<16, true>::smem(SwapCfg<16, true>::STAGES))
+                          : t->nt == 16 ? cudaFuncSetAttribute(k_fp8_swap<16, false>, dyn, SwapCfg<16, false>::smem(SwapCfg<16, false>::STAGES))
+                          : t->nt == 32 ? cudaFuncSetAttribute(k_fp8_swap<32, false>, dyn, SwapCfg<32, false>::smem(SwapCfg<32, false>::STAGES))
+                          : t->nt == 64 ? cudaFuncSetAttribute(k_fp8_swap<64, false>, dyn, SwapCfg<64, false>::smem(SwapCfg<64, false>::STAGES))
+                                        : cudaFuncSetAttribute(k_fp8_swap<128, false>, dyn, SwapCfg<128, false>::smem(SwapCfg<128, false>::STAGES));
     if (e != cudaSuccess) return -1;
     if (encode_rows(&t->mapW, codes, (size_t)p->ob * p->kb * FP8_BLOCK, t->pairs ? 64 : FP8_BLOCK)) return -1;
     return encode_rows(&t->mapX, q, (size_t)p->kb * p->n, t->nt);
@@ -749,8 +768,9 @@ static int cluster_launch(void (*kernel)(KArgs...), unsigned grid, unsigned bloc
 template <int NT, bool FUSE> static int swap_launch(cudaStream_t st, const Fp8Tensor *t, const Fp8Params *p)
 {
     using C = SwapCfg<NT, FUSE>;
-    return cluster_launch(k_fp8_swap<NT, FUSE>, (unsigned)(p->ob * ((p->n + NT - 1) / NT) * t->split), C::THREADS, t->split, C::SMEM, st, t->mapW, t->mapX, *p,
-                          t->split);
+    const int stages = t->stages > C::STAGES ? C::STAGES : t->stages;
+    return cluster_launch(k_fp8_swap<NT, FUSE>, (unsigned)(p->ob * ((p->n + NT - 1) / NT) * t->split), C::THREADS, t->split, C::smem(stages), st, t->mapW,
+                          t->mapX, *p, t->split, stages);
 }
 
 int drk_fp8_tensor_launch(cudaStream_t st, const Fp8Tensor *t, const Fp8Params *p)
