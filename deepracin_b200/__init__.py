@@ -11,7 +11,8 @@ fed [C][H][W] buffers and weights are transposed HWIO -> [Cin][Cout][kh][kw]
 
 Additions: ``Graph.batch`` (images per ``apply``; arrays gain a leading batch axis),
 ``Graph.math`` ('fp32' | 'tf32' | 'fp32x3'), ``Graph.conv_algo``, ``Graph.autotune``, ``Graph.cuda_graph``,
-``Graph.feed_overlap``.
+``Graph.feed_overlap``, ``Graph.fp8_fc`` (fully connected layers with 8-bit weights), and ``score`` (log probabilities, entropy and
+top alternatives of an output).
 
 All computation happens in ``libdeepracin.so`` on the GPU; there is no CPU path here.
 """
@@ -47,6 +48,7 @@ class Node:
         self.desc = desc
         self.params = params
         self.variables = variables
+        self.score_buffers = None
         self.out_shape = None
         self.shape = None
         graph.nodes.append(self)
@@ -85,6 +87,7 @@ class Graph:
         self.fuse = True
         self.cuda_graph = False
         self.feed_overlap = False
+        self.fp8_fc = False
         self.prepared = False
 
     def gpu_ms(self, iterations=1):
@@ -111,6 +114,9 @@ class Environment:
 
     def __exit__(self, type, value, traceback):
         shutil.rmtree(self.tmp_path, ignore_errors=True)
+        for graph in self.graphs:
+            for node in graph.nodes:
+                _free_score_buffers(node)
         # graphs that borrowed the environment's stream go first; the graph that created it tears it down last
         owner = self.graph_with_cl_context
         for graph in self.graphs:
@@ -158,6 +164,7 @@ def prepare(graph):
     lib.dR_setFusion(graph.ptr, 1 if graph.fuse else 0)
     lib.dR_setCudaGraph(graph.ptr, 1 if graph.cuda_graph else 0)
     lib.dR_setFeedOverlap(graph.ptr, 1 if graph.feed_overlap else 0)
+    lib.dR_setFp8FullyConnected(graph.ptr, 1 if graph.fp8_fc else 0)
     if env.graph_with_cl_context == -1:
         model_path = graph.model_path if graph.model_path is not None else env.model_path
         os.makedirs(model_path, exist_ok=True)
@@ -207,6 +214,57 @@ def apply(graph):
     if not lib.dR_apply(graph.ptr):
         raise RuntimeError("DR Error: deepRACIN apply failed!")
     return fetch(graph)
+
+
+def _free_score_buffers(node):
+    if node.score_buffers is not None:
+        for mem in node.score_buffers[1]:
+            lib.dR_clMemoryBufferCleanup(node.graph.ptr, mem)
+        node.score_buffers = None
+
+
+def score(node, labels=None, k=5, scale=1.0):
+    """Scores of an output node's values after ``apply``, at a temperature of 1 / scale: the node's tensor is one row of logits per
+    image (in [C][H][W] order).  labels: integers [batch] or [batch, m] (negative: none given).  Returns the labels' log
+    probabilities (in the shape of ``labels``; None without them), the entropies [batch], and the log probabilities and indices
+    [batch, k] of the k <= 32 largest, descending, equal ones by ascending index.  Blocking."""
+    graph = node.graph
+    if not graph.prepared or node not in graph.outnodes:
+        raise RuntimeError("DR Error: score() needs a prepared graph and a node that is marked as output!")
+    n, length = int(graph.batch), int(np.prod(node.out_shape))
+    if not 0 <= k <= min(32, length):
+        raise ValueError("DR Error: score() gives 0 to min(32, %d) alternatives, not %d!" % (length, k))
+    lab = np.zeros((n, 0), np.int32)
+    if labels is not None:
+        given = np.asarray(labels)
+        if given.dtype.kind not in "iu" or given.ndim not in (1, 2) or given.shape[0] != n:
+            raise TypeError("DR Error: score()'s labels need to be integers [%d] or [%d, m]!" % (n, n))
+        lab = np.ascontiguousarray(np.clip(given.reshape(n, -1), -1, length), np.int32)
+    m = lab.shape[1]
+    if node.score_buffers is None or node.score_buffers[0] != (n, m, k):
+        _free_score_buffers(node)
+        mems = []
+        node.score_buffers = ((n, m, k), mems)
+        for size in (n * m, n * m, n, n * k, n * k):
+            mem = c_void_p()
+            if not lib.dR_createFloatBuffer(graph.ptr, byref(mem), max(size, 1), 0):
+                _free_score_buffers(node)
+                raise RuntimeError("DR Error: score() could not allocate its buffers!")
+            mems.append(mem)
+    d_lab, d_lp, d_h, d_top, d_idx = node.score_buffers[1]
+    if m:
+        lib.dR_uploadArray(graph.ptr, b"labels", lab.ctypes.data_as(c_void_p), 0, lab.nbytes, d_lab)
+    if not lib.dR_scoreNode(graph.ptr, node.ptr, float(scale), d_lab if m else None, m, d_lp if m else None, d_h, k, d_top if k else None, d_idx if k else None):
+        raise RuntimeError("DR Error: score() failed!")
+
+    def get(mem, shape, dtype):
+        a = np.empty(shape, dtype)
+        if a.size:
+            lib.dR_downloadArray(graph.ptr, b"score", byref(mem), 0, a.nbytes, a.ctypes.data_as(c_void_p))
+        return a
+
+    lp = None if labels is None else get(d_lp, (n, m), np.float32).reshape(np.asarray(labels).shape)
+    return lp, get(d_h, (n,), np.float32), get(d_top, (n, k), np.float32), get(d_idx, (n, k), np.int32)
 
 
 def mark_as_output(node):

@@ -73,6 +73,8 @@ _SIGS = {
     "dR_setFusion": (c_int, [c_void_p, c_int]),
     "dR_setCudaGraph": (c_int, [c_void_p, c_int]),
     "dR_setFeedOverlap": (c_int, [c_void_p, c_int]),
+    "dR_setFp8FullyConnected": (c_int, [c_void_p, c_int]),
+    "dR_scoreNode": (c_int, [c_void_p, c_void_p, c_float, c_void_p, c_int, c_void_p, c_void_p, c_int, c_void_p, c_void_p]),
     "dR_setDevice": (c_int, [c_void_p, c_int]),
     "dR_synchronize": (c_int, [c_void_p]),
     "dR_applyTimed": (c_double, [c_void_p, c_int]),

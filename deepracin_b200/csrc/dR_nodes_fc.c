@@ -96,6 +96,15 @@ gboolean dR_fc_createKernel(dR_Graph *net, dR_Node *layer)
     /* tensor modes, batches of 16..128: split-K GEMM on the tensor cores (2: with three-pass, FP32-accurate products); otherwise
        the FP32 weight-streaming kernels */
     fc->chosenTensor = 0;
+    if (net->config->fp8FullyConnected) {
+        if (!dRk_fp8_fc_supported(net->config->batchSize, fc->shape.s0, fc->shape.s1)) {
+            g_print("FullyConnected Layer %d: %d x %d at batch %d is outside the range of 8-bit weights\n", layer->layerID, fc->shape.s0, fc->shape.s1, net->config->batchSize);
+            return FALSE;
+        }
+        fc->chosenTensor = 3;
+        layer->scratchFloats = (dRk_fp8_fc_scratch_bytes(net->config->batchSize, fc->shape.s0, fc->shape.s1) + 3) / 4;
+        return TRUE;
+    }
     if (net->config->mathMode != DR_MATH_FP32 && dRk_tensor_fc_supported(net->config->batchSize, fc->shape.s0, fc->shape.s1))
         fc->chosenTensor = net->config->mathMode == DR_MATH_FP32_TENSOR ? 2 : 1;
     layer->scratchFloats = fc->chosenTensor == 2 ? dRk_tensor_fc_x3_scratch_floats(net->config->batchSize, fc->shape.s0, fc->shape.s1)
@@ -109,7 +118,8 @@ gboolean dR_fc_allocateBuffers(dR_Graph *net, dR_Node *layer)
     dR_FC_Data *fc = (dR_FC_Data *)layer->layer;
     gboolean ret;
     if (!fc->hasVariables) { g_print("FullyConnected Layer %d has no weights (call dR_FullyConnected_setVariables)\n", layer->layerID); return FALSE; }
-    if (fc->chosenTensor) ret = dR_createFloatBufferL(net, &fc->weightsBufT, (fc->chosenTensor == 2 ? 2 : 1) * dRk_tensor_fc_packed_floats(fc->shape.s0, fc->shape.s1));
+    if (fc->chosenTensor == 3) ret = dR_createFloatBufferL(net, &fc->weightsBufQ, (dRk_fp8_fc_packed_bytes(fc->shape.s0, fc->shape.s1) + 3) / 4);
+    else if (fc->chosenTensor) ret = dR_createFloatBufferL(net, &fc->weightsBufT, (fc->chosenTensor == 2 ? 2 : 1) * dRk_tensor_fc_packed_floats(fc->shape.s0, fc->shape.s1));
     else ret = dR_createFloatBufferL(net, &fc->weightsBuf, (size_t)fc->shape.s0 * fc->shape.s1);
     if (fc->useBias) ret &= dR_createFloatBuffer(net, &fc->biasBuf, fc->shape.s1, CL_MEM_READ_ONLY);
     return ret;
@@ -119,7 +129,17 @@ gboolean dR_fc_fillBuffers(dR_Graph *net, dR_Node *layer)
 {
     dR_FC_Data *fc = (dR_FC_Data *)layer->layer;
     gboolean ret;
-    if (fc->chosenTensor) {
+    if (fc->chosenTensor == 3) {
+        /* rounded on the device, from a copy of the float weights that goes when the codes are there */
+        ret = TRUE;
+        if (!net->config->dryRun) {
+            const size_t floats = (size_t)fc->shape.s0 * fc->shape.s1;
+            cl_mem w = NULL;
+            ret = dR_createFloatBufferL(net, &w, floats) && dR_uploadArray(net, "", fc->weights, 0, floats * sizeof(cl_float), w) &&
+                  dRk_fp8_fc_pack_weights(net->clConfig->clCommandQueue, (const float *)w, fc->weightsBufQ, fc->shape.s0, fc->shape.s1) == 0 && dR_finish(net);
+            if (w) { ret &= dR_clMemoryBufferCleanup(net, w); net->clConfig->memConsumptionGPU -= (glong)(floats * sizeof(cl_float)); }
+        }
+    } else if (fc->chosenTensor) {
         /* block-by-block packing for the TMA-fed B operand */
         const size_t np = (fc->chosenTensor == 2 ? 2 : 1) * dRk_tensor_fc_packed_floats(fc->shape.s0, fc->shape.s1);
         gfloat *t = (gfloat *)g_malloc(np * sizeof(gfloat));
@@ -141,6 +161,19 @@ gboolean dR_fc_compute(dR_Graph *net, dR_Node *layer)
     dR_Node *in = dR_firstInput(layer);
     if (in->act_cstride != in->oshape.s2) { g_print("FullyConnected Layer %d: input must be dense\n", layer->layerID); return FALSE; }
     dR_beginCLKernel(net);
+    if (fc->chosenTensor == 3) {
+        /* a feed buffer may have been replaced since the last apply */
+        if (fc->fp8Plan && (fc->fp8In != dR_actPtr(in) || fc->fp8Out != dR_actPtr(layer))) { dRk_fp8_fc_free((dRk_Fp8FcPlan *)fc->fp8Plan); fc->fp8Plan = NULL; }
+        if (!fc->fp8Plan) {
+            fc->fp8In = dR_actPtr(in);
+            fc->fp8Out = dR_actPtr(layer);
+            fc->fp8Plan = dRk_fp8_fc_plan(fc->fp8In, DRK_F32, fc->shape.s0, fc->weightsBufQ, fc->useBias ? (const float *)fc->biasBuf : NULL, fc->fp8Out, DRK_F32,
+                                          fc->shape.s1, net->scratch, net->config->batchSize, fc->shape.s0, fc->shape.s1, fc->activation == tReLU ? 1 : 0, (int *)net->statusWord);
+            if (!fc->fp8Plan) { g_print("FullyConnected Layer %d: 8-bit plan could not be built\n", layer->layerID); return FALSE; }
+        }
+        net->clConfig->clError = dRk_fp8_fc_run(net->clConfig->clCommandQueue, (dRk_Fp8FcPlan *)fc->fp8Plan);
+        return dR_finishCLKernel(net, "deepRACIN:FullyConnected");
+    }
     if (fc->chosenTensor) {
         if (!fc->tmaDescs) {
             fc->tmaDescs = (fc->chosenTensor == 2 ? dRk_tensor_fc_x3_plan : dRk_tensor_fc_plan)(
@@ -163,6 +196,8 @@ gboolean dR_fc_cleanupBuffers(dR_Graph *net, dR_Node *layer)
     gboolean ret = TRUE;
     if (fc->weightsBuf) { ret &= dR_clMemoryBufferCleanup(net, fc->weightsBuf); fc->weightsBuf = NULL; }
     if (fc->weightsBufT) { ret &= dR_clMemoryBufferCleanup(net, fc->weightsBufT); fc->weightsBufT = NULL; }
+    if (fc->weightsBufQ) { ret &= dR_clMemoryBufferCleanup(net, fc->weightsBufQ); fc->weightsBufQ = NULL; }
+    if (fc->fp8Plan) { dRk_fp8_fc_free((dRk_Fp8FcPlan *)fc->fp8Plan); fc->fp8Plan = NULL; }
     if (fc->tmaDescs) { dRk_tensor_fc_free((dRk_TensorFcPlan *)fc->tmaDescs); fc->tmaDescs = NULL; }
     if (fc->biasBuf) { ret &= dR_clMemoryBufferCleanup(net, fc->biasBuf); fc->biasBuf = NULL; }
     return ret;

@@ -349,6 +349,18 @@ gboolean dR_setFusion(dR_Graph *net, gboolean on) { if (!beforePrepare(net, "dR_
 gboolean dR_setFeedOverlap(dR_Graph *net, gboolean on) { if (!beforePrepare(net, "dR_setFeedOverlap")) return FALSE; net->config->feedOverlap = on; return TRUE; }
 gboolean dR_setCudaGraph(dR_Graph *net, gboolean on) { if (!beforePrepare(net, "dR_setCudaGraph")) return FALSE; net->config->useCudaGraph = on; return TRUE; }
 
+gboolean dR_setFp8FullyConnected(dR_Graph *net, gboolean on) { if (!beforePrepare(net, "dR_setFp8FullyConnected")) return FALSE; net->config->fp8FullyConnected = on; return TRUE; }
+
+gboolean dR_scoreNode(dR_Graph *net, dR_Node *node, gfloat scale, const gint *labels, gint numLabels, gfloat *logprob, gfloat *entropy,
+                      gint k, gfloat *topLogprob, gint *topIndex)
+{
+    if (!net->prepared || net->config->dryRun) { g_print("dR_scoreNode: call dR_prepare (with a device) first!\n"); return FALSE; }
+    if (!node || !node->output) { g_print("dR_scoreNode: the node must be marked as output\n"); return FALSE; }
+    const gint length = node->oshape.s0 * node->oshape.s1 * node->oshape.s2;
+    return dRk_logprobs(net->clConfig->clCommandQueue, *node->outputBuf->bufptr, DRK_F32, length, net->config->batchSize, length, scale, labels, numLabels,
+                        logprob, entropy, k, topLogprob, topIndex) == 0;
+}
+
 gboolean dR_setDevice(dR_Graph *net, gint ordinal)
 {
     if (!beforePrepare(net, "dR_setDevice") || ordinal < 0) return FALSE;

@@ -24,6 +24,19 @@ enum dR_InterfaceLayout {
 gboolean dR_setBatchSize(dR_Graph *net, gint n);
 gboolean dR_setMathMode(dR_Graph *net, gint mode);
 gboolean dR_setInterfaceLayout(dR_Graph *net, gint layout);
+/* Fully connected layers with weights in 8-bit floating point (e4m3, a scale per 128 x 128 block; dRk_fp8_fc_* in dR_kernels.h):
+ * a quarter of the weight bytes, products on the tensor cores at any batch size, whatever the math mode.  The weights are rounded
+ * when the graph is prepared, each layer's input when it runs; a saved graph keeps the float weights.  Off by default: operands
+ * then have 4 significant bits, and outputs differ from the float layer's by a few percent of their typical size.  Before
+ * dR_prepare. */
+gboolean dR_setFp8FullyConnected(dR_Graph *net, gboolean on);
+/* Scores of an output node's values after dR_apply, enqueued on the graph's stream (dRk_logprobs in dR_kernels.h): each image's
+ * tensor is one row of logits, in the interface layout's order, at the temperature 1 / scale.  All pointers are device memory:
+ * labels [batch][numLabels] (NULL with numLabels 0), logprob the same shape, entropy [batch] or NULL, topLogprob and topIndex
+ * [batch][k] with k <= min(32, length).  The node must be marked as output; a Softmax node's values are probabilities, so score
+ * the layer in front of it.  FALSE, with a message, for anything it refuses. */
+gboolean dR_scoreNode(dR_Graph *net, dR_Node *node, gfloat scale, const gint *labels, gint numLabels, gfloat *logprob, gfloat *entropy,
+                      gint k, gfloat *topLogprob, gint *topIndex);
 /* Force a kernel family for one convolution node (dR_ConvAlgo); DR_CONV_AUTO restores the rule. */
 gboolean dR_setConvAlgo(dR_Node *node, gint algo);
 /* Graph-wide override, and switch for timing the legal variants of every conv during dR_prepare. */

@@ -20,8 +20,11 @@ struct dR_FC_Data {
     cl_mem weightsBufT;         /* [Nout][Nin] packing for the tensor-core path */
     cl_mem biasBuf;
     gint splitK;                /* K partitions of the weight-streaming kernel (partials live in scratch) */
-    gint chosenTensor;
+    gint chosenTensor;          /* 0 FP32 kernels, 1 TF32, 2 three-pass TF32, 3 e4m3 with block scales */
     void *tmaDescs;
+    cl_mem weightsBufQ;         /* e4m3 packing with its block scales */
+    void *fp8Plan;
+    float *fp8In, *fp8Out;      /* the addresses fp8Plan was made for */
 };
 
 #ifdef __cplusplus

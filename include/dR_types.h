@@ -189,6 +189,7 @@ struct dR_Config {
     gboolean fuseGraph;      /* enable concat elision / preamble folding */
     gboolean useCudaGraph;   /* replay the node schedule from a captured CUDA graph */
     gboolean feedOverlap;    /* dR_feedDataAsync copies on a second stream into alternating buffers */
+    gboolean fp8FullyConnected; /* fully connected layers keep their weights in e4m3 with block scales (dR_setFp8FullyConnected) */
     gboolean dryRun;         /* plan only: no device is touched, buffers get placeholder addresses, dR_apply refuses */
     size_t dryRunCursor;
 };

@@ -1,6 +1,7 @@
 """Refusals of the operator entry points, on the host: every call here is refused before anything is launched."""
 import ctypes
 
+import numpy as np
 import pytest
 
 import deepracin_b200 as dr
@@ -70,3 +71,40 @@ def test_logprobs_refuses(change, says, capfd):
     assert logprobs(**change) == -1
     err = capfd.readouterr().err
     assert err.startswith("dRk_logprobs: ") and says in err
+
+
+def dry_graph(batch, fp8, dims=(300, 200, 40)):
+    env = dr.Environment().__enter__()
+    g = env.create_graph("CHW")
+    x = dr.feed_node(g, [dims[0], 1, 1])
+    node = x
+    for nin, nout in zip(dims, dims[1:]):
+        node = dr.Fully_Connected(node, [nin, nout], "relu", np.zeros((nin, nout), np.float32), np.zeros(nout, np.float32))
+    dr.mark_as_output(node)
+    lib.dR_setBatchSize(g.ptr, batch)
+    assert lib.dR_setFp8FullyConnected(g.ptr, fp8)
+    lib.dR_config(g.ptr, b"", 1, 0, 0, 0, b"")
+    lib.dR_setDryRun(g.ptr, 1)
+    assert lib.dR_prepare(g.ptr)
+    return env, g, node
+
+
+def test_graph_with_8_bit_layers_plans_its_scratch():
+    env, g, _ = dry_graph(7, 1)
+    need = max(lib.dRk_fp8_fc_scratch_bytes(7, 300, 200), lib.dRk_fp8_fc_scratch_bytes(7, 200, 40))
+    assert lib.dR_getScratchFloats(g.ptr) == (need + 3) // 4
+    assert not lib.dR_setFp8FullyConnected(g.ptr, 0)        # too late
+    env.__exit__(None, None, None)
+    env, g, _ = dry_graph(7, 0)
+    assert lib.dR_getScratchFloats(g.ptr) != (need + 3) // 4
+    env.__exit__(None, None, None)
+
+
+def test_score_node_refuses_without_a_device(capfd):
+    env, g, node = dry_graph(2, 0)
+    assert not lib.dR_scoreNode(g.ptr, node.ptr, 1.0, None, 0, None, P, 0, None, None)
+    env.__exit__(None, None, None)
+    with dr.Environment() as env:
+        g = env.create_graph("CHW")
+        x = dr.feed_node(g, [4, 1, 1])
+        assert not lib.dR_scoreNode(g.ptr, x.ptr, 1.0, None, 0, None, P, 0, None, None)
