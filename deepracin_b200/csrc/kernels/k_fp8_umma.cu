@@ -720,18 +720,19 @@ static int encode_rows(CUtensorMap *map, const void *base, size_t rows, int box_
 
 int drk_fp8_tensor_plan(Fp8Tensor *t, const Fp8Params *p, const void *codes, const void *q, int sms)
 {
-    t->pairs = 0;
-    if (p->n > 128) {
-        t->mtiles = (p->n + 255) / 256;
-        t->ntiles = (p->ob + 1) / 2;
-        t->pairs = t->mtiles * t->ntiles < sms / 2 ? t->mtiles * t->ntiles : sms / 2;
-    }
     t->nt = p->n <= 16 ? 16 : p->n <= 32 ? 32 : p->n <= 64 ? 64 : 128;
     /* as many shares of a tile's blocks as still run at once, one on an SM */
     const int tiles = p->ob * ((p->n + t->nt - 1) / t->nt), room = sms;
     t->split = 1;
     while (t->split < 8 && tiles * t->split * 2 <= room && t->split * 4 <= p->kb) t->split *= 2;
     t->stages = (p->kb + t->split - 1) / t->split;
+    /* Above 64 rows a block of 128 inputs takes a CTA of k_fp8_swap<128> 0.62 us and a pair of k_fp8_pair, on four times the tile,
+       0.49 us, and the pair starts 1 us later (4096 -> 4096: 256 rows 21 against 26 us, 384 rows 32 against 27 us; 8192 -> 8192,
+       256 rows: 50 against 42 us).  Rounds times blocks decide. */
+    t->mtiles = (p->n + 255) / 256;
+    t->ntiles = (p->ob + 1) / 2;
+    const long long ptiles = (long long)t->mtiles * t->ntiles, rounds = ((long long)tiles * t->split + sms - 1) / sms, prounds = (ptiles + sms / 2 - 1) / (sms / 2);
+    t->pairs = p->n > 64 && 4 * prounds * p->kb + 8 <= 5 * rounds * t->stages ? (int)(ptiles < sms / 2 ? ptiles : sms / 2) : 0;
     t->fuse = !t->pairs && p->n <= FUSE_ROWS;
     /* the attribute holds for the current device, which is the plan's */
     const cudaFuncAttribute dyn = cudaFuncAttributeMaxDynamicSharedMemorySize;

@@ -104,7 +104,9 @@ def check(got, xq, w, bias, act, kb):
 
 SHAPES = [(1, 1, 1), (1, 128, 128), (2, 129, 127), (3, 127, 257), (5, 16, 3), (16, 256, 384), (17, 1000, 100), (37, 1003, 517),
           (33, 2176, 1000), (64, 4096, 1000), (65, 640, 130), (96, 1500, 129), (128, 384, 256), (129, 300, 200), (200, 2049, 260),
-          (256, 512, 512), (300, 1024, 640), (513, 256, 1000), (1000, 512, 300), (1, 25088, 384), (1030, 1290, 2060), (2500, 384, 515)]
+          (256, 512, 512), (300, 1024, 640), (513, 256, 1000), (1000, 512, 300), (1, 25088, 384), (1030, 1290, 2060), (2500, 384, 515),
+          # pairs of CTAs on 256 x 256 tiles: ragged edges, an odd number of weight blocks, one block, several tiles for each pair
+          (129, 2000, 8200), (333, 3000, 4100), (1500, 1290, 2300), (2100, 900, 1100), (2500, 300, 8200), (3000, 100, 5000)]
 
 
 @pytest.mark.parametrize("types", [(F32, F32), (BF16, BF16), (F16, F32), (F32, F16)])
@@ -123,7 +125,7 @@ def test_against_the_definition(n, nin, nout, types):
     check(layer.result(), quantized(x), dequantized(codes, scales), bias, act, -(-nin // 128))
 
 
-@pytest.mark.parametrize("n,nin,nout", [(1, 700, 300), (37, 1003, 517), (300, 520, 389), (1100, 650, 1300)])
+@pytest.mark.parametrize("n,nin,nout", [(1, 700, 300), (37, 1003, 517), (300, 520, 389), (1100, 650, 1300), (1500, 1290, 2301)])
 @pytest.mark.parametrize("tin,tout", [(F32, F32), (BF16, F16)])
 def test_pitches_and_alignment(n, nin, nout, tin, tout):
     """rows further apart than they are long, starting off every vector boundary; what lies between the rows stays"""
@@ -178,7 +180,7 @@ def test_codes_with_a_row_pitch_and_packing_of_the_float_matrix():
     assert torch.equal(packed[kb * ob * 16384:].view(torch.float32), again[kb * ob * 16384:].view(torch.float32))
 
 
-@pytest.mark.parametrize("n,nin,nout", [(4, 384, 200), (40, 384, 200), (700, 384, 400)])
+@pytest.mark.parametrize("n,nin,nout", [(4, 384, 200), (40, 384, 200), (700, 384, 400), (2100, 1408, 1100)])
 def test_rows_of_zeros_infinities_and_nan(n, nin, nout):
     g = torch.Generator().manual_seed(n)
     x = torch.randn(n, nin, generator=g).cuda()
@@ -194,7 +196,7 @@ def test_rows_of_zeros_infinities_and_nan(n, nin, nout):
     assert bool((got[0] == 0).all())
     assert bool(got[1].isnan().all()) and bool(got[2].isnan().all())
     fine = torch.tensor([0] + list(range(3, n)), device="cuda")
-    check(got[fine], quantized(x[fine]), dequantized(codes, scales), None, 0, 3)
+    check(got[fine], quantized(x[fine]), dequantized(codes, scales), None, 0, nin // 128)
     relu = Layer(x, codes, scales, None, F32, 1)
     relu.run()
     assert bool(relu.result()[2].isnan().all())
@@ -211,7 +213,7 @@ def test_nan_weights_stay_in_their_column():
 
 
 def test_same_answer_every_time_and_after_other_work():
-    for n, nin, nout in [(1, 4096, 512), (50, 2048, 512), (600, 1024, 512)]:
+    for n, nin, nout in [(1, 4096, 512), (50, 2048, 512), (600, 1024, 512), (2100, 1024, 1100)]:
         codes, scales = make_weights(nin, nout, 2)
         x = torch.randn(n, nin, device="cuda")
         layer = Layer(x, codes, scales, None, F32, 0)
@@ -226,7 +228,7 @@ def test_same_answer_every_time_and_after_other_work():
 
 def test_streams_and_graph_capture():
     """two plans at once on two streams; a plan captured, replayed on new inputs; a plan on a stream other than torch's"""
-    shapes = [(1, 4096, 1000), (64, 2048, 640), (520, 1024, 700)]
+    shapes = [(1, 4096, 1000), (64, 2048, 640), (520, 1024, 700), (2100, 1024, 1100)]
     for n, nin, nout in shapes:
         codes, scales = make_weights(nin, nout, 9)
         w = dequantized(codes, scales)
