@@ -180,7 +180,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) k_logprobs(const LpParams p)
         if (label >= 0 && label < p.len) labelled = Y::one(v + label);
     }
 
-    float m = -INFINITY, S0 = 0.0f, S1 = 0.0f, T0 = 0.0f, T1 = 0.0f, mine = -INFINITY;
+    float m = -INFINITY, RS = 0.0f, RT = 0.0f, mine = -INFINITY;
     const int batches = (count + NT * LP_U - 1) / (NT * LP_U), per_slot = max(1, (batches + LP_SLOTS - 1) / LP_SLOTS);
     uint4 next[LP_U];
     auto fetch = [&](int b) {
@@ -205,10 +205,11 @@ __global__ void __launch_bounds__(NT, 1024 / NT) k_logprobs(const LpParams p)
             const float bm = Y::last(w2);
             sm = lp_max_nan(sm, bm);
             if (bm > m) {
-                lp_rescale((bm - m) * c, S0, T0);
-                lp_rescale((bm - m) * c, S1, T1);
+                lp_rescale((bm - m) * c, RS, RT);
                 m = bm;
             }
+            /* a batch is summed by itself: a long row adds len / (threads x 16 or 32) of them, not its values, to one sum */
+            float s0 = 0.0f, s1 = 0.0f, t0 = 0.0f, t1 = 0.0f;
 #pragma unroll
             for (int u = 0; u < LP_U; u++) {
                 float x[V];
@@ -217,27 +218,27 @@ __global__ void __launch_bounds__(NT, 1024 / NT) k_logprobs(const LpParams p)
                 for (int j = 0; j < V; j += 2) {
                     const float d0 = fmaxf((x[j] - m) * c, LP_LOW), d1 = fmaxf((x[j + 1] - m) * c, LP_LOW);    /* NaN: LP_LOW too */
                     const float e0 = lp_exp2(d0), e1 = lp_exp2(d1);
-                    S0 += e0; S1 += e1;
-                    T0 = fmaf(e0, d0, T0); T1 = fmaf(e1, d1, T1);
+                    s0 += e0; s1 += e1;
+                    t0 = fmaf(e0, d0, t0); t1 = fmaf(e1, d1, t1);
                 }
             }
+            RS += s0 + s1;
+            RT += t0 + t1;
         }
         smax[slot][tid] = sm;
         mine = lp_max_nan(mine, sm);
     }
-    S0 += S1;
-    T0 += T1;
     uint32_t own_single = 0;                /* order of the single value this thread looks at */
     if (tid < singles) {
         const float x = Y::one(v + single_index(tid));
         own_single = lp_order(x);
         if (x > m) {
-            lp_rescale((x - m) * c, S0, T0);
+            lp_rescale((x - m) * c, RS, RT);
             m = x;
         }
         const float d = fmaxf((x - m) * c, LP_LOW), e = lp_exp2(d);
-        S0 += e;
-        T0 = fmaf(e, d, T0);
+        RS += e;
+        RT = fmaf(e, d, RT);
     }
     const uint32_t own = tid < count ? lp_order(mine) : 0;      /* order of the largest of this thread's vectors */
 
@@ -256,9 +257,9 @@ __global__ void __launch_bounds__(NT, 1024 / NT) k_logprobs(const LpParams p)
     __syncthreads();
 #pragma unroll
     for (int w = 0; w < WARPS; w++) { M = fmaxf(M, fred[0][w]); O = max(O, __float_as_uint(fred[1][w])); }
-    lp_rescale((M - m) * c, S0, T0);
-    for (int o = 16; o > 0; o >>= 1) { S0 += __shfl_xor_sync(0xffffffffu, S0, o); T0 += __shfl_xor_sync(0xffffffffu, T0, o); }
-    if (lane == 0) { fred[2][warp] = S0; fred[3][warp] = T0; }
+    lp_rescale((M - m) * c, RS, RT);
+    for (int o = 16; o > 0; o >>= 1) { RS += __shfl_xor_sync(0xffffffffu, RS, o); RT += __shfl_xor_sync(0xffffffffu, RT, o); }
+    if (lane == 0) { fred[2][warp] = RS; fred[3][warp] = RT; }
     /* the k-th largest group */
     if (p.k > 0 && tid < LP_GROUPS) {
         const uint32_t x = group[tid];
@@ -484,7 +485,7 @@ extern "C" int dRk_logprobs(dRk_stream stream, const void *logits, int type, lon
     if (n > 1 && ld < len) return lp_refuse("rows overlap (ld < len)");
     if (m < 0 || k < 0 || k > LP_KMAX || k > len) return lp_refuse("number of labels below 0, or of alternatives outside 0..min(32, len)");
     if (!logits || (m > 0 && (!labels || !logprob)) || (k > 0 && (!top_logprob || !top_index))) return lp_refuse("null pointer");
-    if (!(scale > 0.0f) || isinf(scale)) return lp_refuse("scale (1 / temperature) must be positive and finite");
+    if (!(scale > 0.0f) || !(scale <= 0x1p120f)) return lp_refuse("scale (1 / temperature) must be positive and at most 2^120");
     if ((uintptr_t)logits % size || (uintptr_t)labels % 4 || (uintptr_t)logprob % 4 || (uintptr_t)entropy % 4 || (uintptr_t)top_logprob % 4 || (uintptr_t)top_index % 4)
         return lp_refuse("pointer not aligned to its element type");
     const int dev = drk_stream_device("dRk_logprobs", stream, -1);

@@ -243,12 +243,14 @@ enum { DRK_F32 = 0, DRK_BF16 = 1, DRK_F16 = 2 };
  * only (Kernels/dR_fcl.cl:59-120); an output's error against dRk_fc_f32 is that of operands with 4 significant bits.
  *   in  : n rows of Nin values of in_type, ldi elements apart;  out : n rows of Nout values of out_type, ldo elements apart
  *         (what lies between Nout and ldo is left as it is);  bias : Nout floats or NULL;  act : 0 linear, 1 ReLU (NaN passes)
+ *         (out must not overlap in; what leaves the range of a 16-bit out_type becomes an infinity)
  *   packed : dRk_fp8_fc_packed_bytes() bytes, scratch : dRk_fp8_fc_scratch_bytes() bytes, both on 16-byte boundaries.
  * A row that holds an infinity or a NaN becomes NaN; the other rows do not see it.
  * A plan keeps the pointers it was made with and belongs to the device that was current; run refuses another one, or another
  * device's stream (-6).  Runs of plans that share a scratch or an output must not overlap on the GPU; neither must two runs of
  * one plan on two streams.  A run only enqueues (two launches), allocates nothing and may be captured into a CUDA graph.
- * `status` (may be NULL) as dRk_tensor_conv_plan.  _plan returns NULL, the others a negative value, with a message on stderr,
+ * The packed weights are read ahead of the launch in front: write them with the calls below, copies, or kernels without an early
+ * programmatic trigger.  `status` (may be NULL) as dRk_tensor_conv_plan.  _plan returns NULL, the others a negative value, with a message on stderr,
  * for arguments that they refuse.
  */
 typedef struct dRk_Fp8FcPlan dRk_Fp8FcPlan;
@@ -274,7 +276,7 @@ void dRk_fp8_fc_free(dRk_Fp8FcPlan *plan);
  *   top_logprob, top_index [n][k]  the k <= min(32, len) largest logits, descending, equal ones by ascending index, NaN first
  * Logits of -inf have probability 0 (a mask); a row of nothing else scores -inf everywhere, its entropy is 0.  A NaN or +inf
  * makes every score of its row NaN (the order of the alternatives stands).  m = 0 and k = 0 are allowed.  Sums are held in 32 bits.  Next to dRk_softmax (src/dR_nodes_math.c:620-678), which writes the probabilities themselves.
- * At most 2^28 rows of 2^30 logits.  One launch, no workspace; -1 (with a message on stderr) for refused arguments, -6 for another device's stream.
+ * At most 2^28 rows of 2^30 logits; 0 < scale <= 2^120.  One launch, no workspace; -1 (with a message on stderr) for refused arguments, -6 for another device's stream.
  */
 int dRk_logprobs(dRk_stream stream, const void *logits, int type, long long ld, int n, int len, float scale, const int *labels, int m,
                  float *logprob, float *entropy, int k, float *top_logprob, int *top_index);

@@ -64,6 +64,8 @@ def check(v, got, labels, k, scale):
     logp = d - logS
 
     def close(got, want, dd, rows):
+        # the outputs are held in 32 bits: what lies beyond their range (2^128 less half a step) rounds to an infinity
+        want = torch.where(want.abs() >= 2.0 ** 128 - 2.0 ** 103, torch.sign(want) * math.inf, want)
         err = (got.double() - want).abs()
         tol = sum_err[:, None] + 2.0 ** -22 * (torch.where(dd.isfinite(), dd, 0.0).abs() + logS.abs())
         good = torch.where(want.isfinite(), err <= tol, got.double() == want)
@@ -162,9 +164,42 @@ def test_masks_infinities_and_nan(length):
     assert float(got[0][1, 0]) == 0.0 and float(got[1][1]) == 0.0
 
 
+@pytest.mark.parametrize("kind", ["equal", "two values", "ascending", "descending", "crowded", "masked"])
+@pytest.mark.parametrize("n,length", [(160, 5000), (150, 33000), (150, 131072)])
+def test_hard_orders_in_rows_of_one_cta(kind, n, length):
+    """more than two rows per SM are not split; crowded: thousands of the largest values in the shares of eight of 256 threads"""
+    k = 32
+    v = torch.randn(n, length, device="cuda")
+    i = torch.arange(length, device="cuda")
+    rows = slice(3, 9)
+    if kind == "equal":
+        v[rows] = 0.25
+    elif kind == "two values":
+        v[rows] = torch.randint(0, 2, (6, length), device="cuda").float()
+    elif kind == "ascending":
+        v[rows] = i.float() / 16
+    elif kind == "descending":
+        v[rows] = -i.float() / 16
+    elif kind == "crowded":
+        v[rows] += 50.0 * ((i // 4) % 256 < 8)
+    else:
+        v[rows, : length - 40] = -math.inf
+    got = call(v, None, k)
+    check(v[rows], [t[rows] for t in got], None, k, 1.0)
+    b = v[:9].repeat(n // 9, 1).half()
+    check(b[:9], [t[:9] for t in call(b, None, k)], None, k, 1.0)
+
+
+def test_very_long_rows():
+    v = torch.randn(2, 3000001, device="cuda") * 2
+    labels = torch.tensor([[0], [3000000]], dtype=torch.int32, device="cuda")
+    check(v, call(v, labels, 20), labels, 20, 1.0)
+
+
 def test_large_logits_and_small_temperatures():
     v = torch.randn(4, 5000, device="cuda") * 1e4
     check(v, call(v, None, 5, 100.0), None, 5, 100.0)
+    check(v, call(v, None, 5, 2.0 ** 120), None, 5, 2.0 ** 120)
     v = torch.randn(4, 5000, device="cuda") * 1e-3 + 1e3
     check(v, call(v, None, 5, 0.01), None, 5, 0.01)
 

@@ -65,7 +65,7 @@ def logprobs(**kw):
     (dict(ld=99), "rows overlap"), (dict(m=-1), "number of labels"), (dict(k=33), "number of labels"), (dict(k=-1), "number of labels"),
     (dict(length=4, ld=4, k=5), "number of labels"), (dict(logits=None), "null pointer"), (dict(labels=None), "null pointer"),
     (dict(logprob=None), "null pointer"), (dict(top=None), "null pointer"), (dict(index=None), "null pointer"),
-    (dict(scale=0.0), "scale"), (dict(scale=-1.0), "scale"), (dict(scale=float("nan")), "scale"), (dict(scale=float("inf")), "scale"),
+    (dict(scale=0.0), "scale"), (dict(scale=-1.0), "scale"), (dict(scale=float("nan")), "scale"), (dict(scale=float("inf")), "scale"), (dict(scale=3e38), "scale"),
     (dict(logits=P + 2), "not aligned"), (dict(type=2, logits=P + 1), "not aligned"), (dict(labels=P + 1), "not aligned"), (dict(entropy=P + 2), "not aligned")])
 def test_logprobs_refuses(change, says, capfd):
     assert logprobs(**change) == -1
