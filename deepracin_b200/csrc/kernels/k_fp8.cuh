@@ -25,10 +25,10 @@ struct Fp8Params {
     const void *in;
     size_t ldi;
     int in_type, Nin, vec;              /* vec: rows of `in` start on 16-byte boundaries */
-    const float *sx, *scales, *bias;    /* sx [n][kbp], scales [ob][kb] */
+    const float *sx, *scales, *bias;    /* sx [kb][n], scales [ob][kb] */
     void *out;
     size_t ldo;
-    int out_type, n, Nout, kb, kbp, ob, act;   /* kbp: kb rounded up to four */
+    int out_type, n, Nout, kb, ob, act;
     int *status;
 };
 

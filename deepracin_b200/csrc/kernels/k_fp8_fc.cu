@@ -25,10 +25,10 @@ __device__ __forceinline__ float fp8_decode(unsigned char c) { return __half2flo
 /* ------------------------------------------------------------------ activations
  * A half warp owns a block of 128 values of one row, 8 per lane, and asks for U blocks before it rounds the first: bound by HBM
  * (reads sizeof(T), writes one byte a value).  4096 x 8192 bf16 with one block under way: 30 us; U = 4: QUANT_BIG.
- * q: [block][n rows][128], sx: [n rows][kbp blocks]. */
+ * q: [block][n rows][128], sx: [block][n rows]. */
 template <typename T, int U>
 __global__ void __launch_bounds__(256) k_fp8_quantize_rows(const T *__restrict__ in, size_t ldi, unsigned char *__restrict__ q, float *__restrict__ sx,
-                                                           int n, int Nin, int kb, int kbp, int vec)
+                                                           int n, int Nin, int kb, int vec)
 {
     drk_dep_wait();
     drk_dep_trigger();
@@ -78,7 +78,7 @@ __global__ void __launch_bounds__(256) k_fp8_quantize_rows(const T *__restrict__
             }
             if (row[u] != 0xffffffffu) {
                 *reinterpret_cast<uint2 *>(q + ((size_t)blk[u] * n + row[u]) * FP8_BLOCK + sub * 8) = make_uint2(c[0], c[1]);
-                if (sub == 0) sx[(size_t)row[u] * kbp + blk[u]] = __fdiv_rn(a, FP8_MAX);
+                if (sub == 0) sx[(size_t)blk[u] * n + row[u]] = __fdiv_rn(a, FP8_MAX);
             }
         }
     }
@@ -183,7 +183,7 @@ extern "C" size_t dRk_fp8_fc_packed_bytes(int Nin, int Nout)
 extern "C" size_t dRk_fp8_fc_scratch_bytes(int n, int Nin, int Nout)
 {
     if (!dRk_fp8_fc_supported(n, Nin, Nout)) return 0;
-    return (size_t)n * (fp8_blocks(Nin) * (size_t)FP8_BLOCK + (size_t)((fp8_blocks(Nin) + 3) & ~3) * sizeof(float));
+    return (size_t)fp8_blocks(Nin) * n * (FP8_BLOCK + sizeof(float));
 }
 
 static int fp8_pack_checks(const char *who, const void *src, const void *packed, int Nin, int Nout)
@@ -265,7 +265,7 @@ extern "C" dRk_Fp8FcPlan *dRk_fp8_fc_plan(const void *in, int in_type, long long
     p->p.out = out;
     p->p.ldo = (size_t)ldo;
     p->p.out_type = out_type;
-    p->p.n = n; p->p.Nout = Nout; p->p.kb = kb; p->p.kbp = (kb + 3) & ~3; p->p.ob = ob; p->p.act = act;
+    p->p.n = n; p->p.Nout = Nout; p->p.kb = kb; p->p.ob = ob; p->p.act = act;
     p->p.status = status;
     int sms = 148;
     if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || drk_fp8_tensor_plan(&p->t, &p->p, codes, p->q, sms)) {
@@ -284,7 +284,7 @@ template <typename T> static int fp8_quantize(const dRk_Fp8FcPlan *p, cudaStream
     const bool many = halves > 4 * 16 * 148 * 4;
     const unsigned blocks = drk_blocks(many ? (halves + 3) / 4 : halves, 16, 148u * 16u);
     return drk_launched(drk_launch_dep(many ? k_fp8_quantize_rows<T, 4> : k_fp8_quantize_rows<T, 1>, dim3(blocks), dim3(256), 0, st, (const T *)p->p.in,
-                                       p->p.ldi, p->q, p->sx, p->p.n, p->p.Nin, p->p.kb, p->p.kbp, p->p.vec));
+                                       p->p.ldi, p->q, p->sx, p->p.n, p->p.Nin, p->p.kb, p->p.vec));
 }
 
 extern "C" int dRk_fp8_fc_run(dRk_stream stream, dRk_Fp8FcPlan *p)

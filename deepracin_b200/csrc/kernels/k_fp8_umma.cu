@@ -6,6 +6,7 @@
  */
 #include <stdlib.h>
 #include <string.h>
+#include <type_traits>
 #include "k_fp8.cuh"
 #include "k_umma.cuh"
 
@@ -57,6 +58,27 @@ __device__ __forceinline__ void tmem_ld_wait(uint32_t taddr, uint32_t (&r)[64])
                    "=r"(r[48]), "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]),
                    "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63])
                  : "r"(taddr) : "memory");
+}
+/* Loads ahead of their use.  They stay where they are written (the compiler would move plain ones down to the use), and callers
+ * clamp addresses instead of skipping a load, and use a register again instead of handing its value on: a copy of a loaded value
+ * waits for the load, be it at the end of a branch or of a loop's pass.  ld_ahead is for what this launch or the one in front
+ * writes, ld_const for weights' scales. */
+__device__ __forceinline__ float ld_ahead(const float *p)
+{
+    float v;
+    asm volatile("ld.global.cg.f32 %0, [%1];" : "=f"(v) : "l"(p));
+    return v;
+}
+__device__ __forceinline__ float ld_const(const float *p)
+{
+    float v;
+    asm volatile("ld.global.nc.f32 %0, [%1];" : "=f"(v) : "l"(p));
+    return v;
+}
+/* two FP32 FMAs in one instruction */
+__device__ __forceinline__ void ffma2(unsigned long long &acc, unsigned long long a, uint32_t b0, uint32_t b1)
+{
+    asm("{\n\t.reg .b64 b;\n\tmov.b64 b, {%2, %3};\n\tfma.rn.f32x2 %0, %1, b, %0;\n\t}" : "+l"(acc) : "l"(a), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ bool elect_one()
 {
@@ -134,11 +156,11 @@ __device__ __forceinline__ bool mbar_wait1(uint32_t bar, uint32_t parity, volati
  * additions -- the wait, the factors -- is 350 of 600 clocks); with NT = 128 each has half of the rows instead.  A block's
  * accumulator is one of SLOTS in TMEM.  The weights do not depend on the launch in front: their first blocks are on the way before it ends.
  *
- * FUSE (at most FUSE_ROWS rows): four more warps round the input themselves, a block each in turn, straight into the swizzled
- * operand tile; what took two launches takes one.
+ * FUSE (the bytes of an input value; at most FUSE_ROWS rows): four more warps round the input themselves, a block each in turn,
+ * straight into the swizzled operand tile; what takes two launches takes one.
  */
 #define FUSE_ROWS 4
-template <int NT, bool FUSE> struct SwapCfg {
+template <int NT, int FUSE> struct SwapCfg {
     static constexpr int B_BYTES = NT * FP8_BLOCK;
     static constexpr int STAGE_BYTES = FP8_BLOCK_BYTES + B_BYTES;
     static constexpr int STAGES = NT == 16 ? 10 : NT == 32 ? 9 : NT == 64 ? 6 : 4;       /* at most: fewer for a short share */
@@ -154,30 +176,25 @@ template <int NT, bool FUSE> struct SwapCfg {
     static constexpr int smem(int stages) { return 1024 + stages * STAGE_BYTES + INBOX * 4 + FACTORS * 4 + 256; }
 };
 
+__device__ __forceinline__ float2 fp8_two(uint32_t w, int type)
+{
+    return type == DRK_BF16 ? make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)) : __half22float2(*reinterpret_cast<const __half2 *>(&w));
+}
 /* four values of a row from k on, zero behind Nin */
 __device__ __forceinline__ float4 fp8_load4(const Fp8Params &p, int r, int k)
 {
-    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    float e[4];
     const size_t at = (size_t)r * p.ldi + k;
-    if (p.vec && k + 4 <= p.Nin) {
-        if (p.in_type == DRK_F32) return __ldg(reinterpret_cast<const float4 *>(static_cast<const float *>(p.in) + at));
-        const uint2 w = __ldg(reinterpret_cast<const uint2 *>(static_cast<const char *>(p.in) + 2 * at));
-        if (p.in_type == DRK_BF16)
-            return make_float4(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u), __uint_as_float(w.y << 16), __uint_as_float(w.y & 0xffff0000u));
-        const float2 a = __half22float2(*reinterpret_cast<const __half2 *>(&w.x)), b = __half22float2(*reinterpret_cast<const __half2 *>(&w.y));
-        return make_float4(a.x, a.y, b.x, b.y);
-    }
-    float *e = &v.x;
 #pragma unroll
     for (int j = 0; j < 4; j++)
-        if (k + j < p.Nin)
-            e[j] = p.in_type == DRK_F32    ? static_cast<const float *>(p.in)[at + j]
-                   : p.in_type == DRK_BF16 ? __bfloat162float(static_cast<const __nv_bfloat16 *>(p.in)[at + j])
-                                           : __half2float(static_cast<const __half *>(p.in)[at + j]);
-    return v;
+        e[j] = k + j >= p.Nin        ? 0.0f
+               : p.in_type == DRK_F32  ? static_cast<const float *>(p.in)[at + j]
+               : p.in_type == DRK_BF16 ? __bfloat162float(static_cast<const __nv_bfloat16 *>(p.in)[at + j])
+                                       : __half2float(static_cast<const __half *>(p.in)[at + j]);
+    return make_float4(e[0], e[1], e[2], e[3]);
 }
 
-template <int NT, bool FUSE>
+template <int NT, int FUSE>
 __global__ void __launch_bounds__((SwapCfg<NT, FUSE>::THREADS), 1)
 k_fp8_swap(const __grid_constant__ CUtensorMap mapW, const __grid_constant__ CUtensorMap mapX, const __grid_constant__ Fp8Params p, int split, int stages)
 {
@@ -286,36 +303,31 @@ k_fp8_swap(const __grid_constant__ CUtensorMap mapW, const __grid_constant__ CUt
         const int quarter = warp & 3, part = (warp - 2) >> 2, c0 = C::GROUPS == 2 ? 0 : part * C::COLS;
         float *mine = factors + (warp - 2) * 2 * C::COLS;
         constexpr int PER = (C::COLS + 31) / 32;
-        float4 now[PER], next[PER];     /* sx of this lane's rows for the blocks of a group of four, and for the next group */
-        float sw = 0.0f, sw_next = 0.0f;
         const float *swp = p.scales + (size_t)ot * p.kb;
         drk_dep_wait();     /* sx is written by the launch in front; the rows in p.out may still be read by it */
-        auto fetch = [&](int b) {
+        const int first = b0 + (C::GROUPS == 2 ? part : 0), last = b1 - 1;      /* this group's first block */
+        /* factors of this group's block and of its next one; rows behind the last stand for the last (they are not stored) */
+        const float *sxp[PER];
+        float x[PER], x1[PER], sw = 0.0f, sw1 = 0.0f;
+        auto fetch = [&](int b, float (&to)[PER]) {
 #pragma unroll
-            for (int j = 0; j < PER; j++) {
-                const int r = c0 + j * 32 + lane;
-                next[j] = j * 32 + lane < C::COLS && r0 + r < p.n ? __ldcg(reinterpret_cast<const float4 *>(p.sx + (size_t)(r0 + r) * p.kbp + (b & ~3)))
-                                                                  : make_float4(0.f, 0.f, 0.f, 0.f);
-            }
+            for (int j = 0; j < PER; j++) to[j] = ld_ahead(sxp[j] + (size_t)min(b, last) * p.n);
+            return ld_const(swp + min(b, last));
         };
-        const int first = b0 + (C::GROUPS == 2 ? part : 0);         /* this group's first block */
-        if (!FUSE && first < b1) { fetch(first); sw_next = __ldg(swp + first); }
+        if (!FUSE) {
+#pragma unroll
+            for (int j = 0; j < PER; j++) sxp[j] = p.sx + min(r0 + c0 + j * 32 + lane, p.n - 1);
+            sw = fetch(first, x);
+            sw1 = fetch(first + C::GROUPS, x1);
+        }
         int slot = C::GROUPS == 2 ? part : 0, flip = 0;
         uint32_t sphase = 0;
         for (int b = first; b < b1; b += C::GROUPS) {
             const float *f = factors + ((b - b0) % C::RING) * NT + c0;
             if (!FUSE) {
                 float *g = mine + flip * C::COLS;
-                if (b == first || (b & 3) < C::GROUPS) {
 #pragma unroll
-                    for (int j = 0; j < PER; j++) now[j] = next[j];
-                    if ((b | 3) + 1 < b1) fetch((b | 3) + 1);
-                }
-                sw = sw_next;
-                if (b + C::GROUPS < b1) sw_next = __ldg(swp + b + C::GROUPS);
-#pragma unroll
-                for (int j = 0; j < PER; j++)
-                    if (j * 32 + lane < C::COLS) g[j * 32 + lane] = ((b & 2) ? ((b & 1) ? now[j].w : now[j].z) : ((b & 1) ? now[j].y : now[j].x)) * sw;
+                for (int j = 0; j < PER; j++) if (j * 32 + lane < C::COLS) g[j * 32 + lane] = x[j] * sw;
                 __syncwarp();
                 f = g;
                 flip ^= 1;
@@ -342,45 +354,71 @@ k_fp8_swap(const __grid_constant__ CUtensorMap mapW, const __grid_constant__ CUt
                     acc[c + j + 3] = fmaf(g.w, __uint_as_float(r[j + 3]), acc[c + j + 3]);
                 }
             }
+            if (!FUSE) {
+#pragma unroll
+                for (int j = 0; j < PER; j++) x[j] = x1[j];
+                sw = sw1;
+                sw1 = fetch(b + 2 * C::GROUPS, x1);
+            }
             slot += C::GROUPS;
             if (slot >= C::SLOTS) { slot -= C::SLOTS; sphase ^= 1u; }
         }
     } else if (FUSE) {
         /* warp w rounds the blocks w, w + 4, ...: a row's 128 values are four per lane */
+        using Raw = typename std::conditional<FUSE == 4, uint4, uint2>::type;
         const float *swp = p.scales + (size_t)ot * p.kb;
-        float4 x[FUSE_ROWS];
-        float sw = 0.0f;
-        int b = b0 + warp - 10;
+        const int first = b0 + warp - 10, last = b1 - 1;
         drk_dep_wait();
-        if (b < b1) {
-            sw = __ldg(swp + b);
+        auto rounding = [&](auto fast) {
+            constexpr bool FAST = decltype(fast)::value;    /* whole vectors: the next block's are on their way while one is rounded */
+            const char *row[FUSE_ROWS];
+            Raw raw[FUSE_ROWS];
+            float sw = 0.0f;
+            auto fetch = [&](int b, int r) {
+                const char *at = row[r] + (size_t)min(min(b, last) * FP8_BLOCK + lane * 4, p.Nin - 4) * FUSE;
+                if constexpr (FUSE == 4) asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(raw[r].x), "=r"(raw[r].y), "=r"(raw[r].z), "=r"(raw[r].w) : "l"(at));
+                else asm volatile("ld.global.v2.u32 {%0, %1}, [%2];" : "=r"(raw[r].x), "=r"(raw[r].y) : "l"(at));
+            };
+            if (FAST) {
 #pragma unroll
-            for (int r = 0; r < FUSE_ROWS; r++) if (r < p.n) x[r] = fp8_load4(p, r, b * FP8_BLOCK + lane * 4);
-        }
-        for (; b < b1; b += 4) {
-            const int i = b - b0, stage = i % stages;
-            const float s = sw;
-            if (b + 4 < b1) sw = __ldg(swp + b + 4);
-            if (i >= stages && !mbar_wait_warp_inline(empty_bar(stage), ((uint32_t)(i / stages) & 1u) ^ 1u, abort_flag, p.status, 35)) break;
-            char *tile_x = gen + stage * C::STAGE_BYTES + FP8_BLOCK_BYTES;
-            float *f = factors + (i % C::RING) * NT;
-#pragma unroll
-            for (int r = 0; r < FUSE_ROWS; r++) {
-                if (r >= p.n) break;
-                const float4 v = x[r];
-                if (b + 4 < b1) x[r] = fp8_load4(p, r, (b + 4) * FP8_BLOCK + lane * 4);
-                float a = fmaxf(fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))), FP8_FLOOR);
-                a = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(a)));      /* positive floats compare as whole numbers */
-                const float inv = __fdiv_rn(FP8_MAX, a);
-                const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(v.x * inv, v.y * inv), __NV_SATFINITE, __NV_E4M3);
-                const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(v.z * inv, v.w * inv), __NV_SATFINITE, __NV_E4M3);
-                *reinterpret_cast<uint32_t *>(tile_x + r * FP8_BLOCK + ((((lane >> 2) ^ (r & 7)) << 4) | ((lane & 3) << 2))) = lo | (hi << 16);
-                if (lane == 0) f[r] = __fdiv_rn(a, FP8_MAX) * s;
+                for (int r = 0; r < FUSE_ROWS; r++) { row[r] = static_cast<const char *>(p.in) + (size_t)min(r, p.n - 1) * p.ldi * FUSE; fetch(first, r); }
             }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) mbar_arrive(full_bar(stage));
-        }
+            sw = ld_const(swp + min(first, last));
+            for (int b = first; b < b1; b += 4) {
+                const int i = b - b0, stage = i % stages;
+                if (i >= stages && !mbar_wait_warp_inline(empty_bar(stage), ((uint32_t)(i / stages) & 1u) ^ 1u, abort_flag, p.status, 35)) break;
+                char *tile_x = gen + stage * C::STAGE_BYTES + FP8_BLOCK_BYTES;
+                float *f = factors + (i % C::RING) * NT;
+#pragma unroll
+                for (int r = 0; r < FUSE_ROWS; r++) {
+                    float4 v;
+                    if constexpr (FAST) {
+                        if constexpr (FUSE == 4) v = make_float4(__uint_as_float(raw[r].x), __uint_as_float(raw[r].y), __uint_as_float(raw[r].z), __uint_as_float(raw[r].w));
+                        else {
+                            const float2 lo = fp8_two(raw[r].x, p.in_type), hi = fp8_two(raw[r].y, p.in_type);
+                            v = make_float4(lo.x, lo.y, hi.x, hi.y);
+                        }
+                        if (b * FP8_BLOCK + lane * 4 >= p.Nin) v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                        fetch(b + 4, r);
+                    }
+                    if (r >= p.n) continue;
+                    if constexpr (!FAST) v = fp8_load4(p, r, b * FP8_BLOCK + lane * 4);
+                    float a = fmaxf(fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))), FP8_FLOOR);
+                    a = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(a)));      /* positive floats compare as whole numbers */
+                    const float inv = __fdiv_rn(FP8_MAX, a);
+                    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(v.x * inv, v.y * inv), __NV_SATFINITE, __NV_E4M3);
+                    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(v.z * inv, v.w * inv), __NV_SATFINITE, __NV_E4M3);
+                    *reinterpret_cast<uint32_t *>(tile_x + r * FP8_BLOCK + ((((lane >> 2) ^ (r & 7)) << 4) | ((lane & 3) << 2))) = lo | (hi << 16);
+                    if (lane == 0) f[r] = __fdiv_rn(a, FP8_MAX) * sw;
+                }
+                sw = ld_const(swp + min(b + 4, last));
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(full_bar(stage));
+            }
+        };
+        if (p.vec && p.Nin % 4 == 0) rounding(std::true_type{});
+        else rounding(std::false_type{});
     }
     drk_dep_trigger();
 
@@ -420,20 +458,24 @@ k_fp8_swap(const __grid_constant__ CUtensorMap mapW, const __grid_constant__ CUt
  * fetches its 128 rows of the input and 64 rows of each of the tile's two weight blocks (32 KiB a stage; a single CTA's tile of
  * 128 x 256 would fetch 48), counted on the leader's barriers.  Two warps of the leader issue, one for each weight block (M = 256,
  * N = 128, four MMAs of K = 32), into one of two accumulators per block; the commits tell both CTAs.  Warps 4-11 own 32 rows and
- * one weight block each: they read the accumulator, hand its slot back, and add it times sx * sw to 128 sums per lane.
+ * one weight block each: they read the accumulator, hand its slot back, and add it times sx * sw to 128 sums per lane.  Warp 3
+ * makes the factors sx * sw of a block and leaves them in shared memory.
  *
- * What bounds it: the way issue -> commit -> read -> hand back -> issue, about 1000 clocks with two accumulators under way, where
- * the MMAs of a block take 512.  4096 x 8192 -> 8192: 290 us with the rounding of the input (1.9 PFLOP/s); without the sums (copy
- * and MMAs alone) 207 us.  Measured on the way there: all sums in one accumulator of 256 columns and one issuing lane 309-320 us;
- * additions as packed FFMA2 over registers that had to be paired up 370 us and more; a cluster-scope release on the hand-back
- * (a memory barrier) 450 us.
+ * What bounds it: the way issue -> commit -> read -> hand back -> issue, 700 to 900 clocks a block with two accumulators under
+ * way, where the MMAs take 512; in a long run the board's power (half of it spent on copies and at rest, a third on the MMAs).
+ * 4096 x 8192 -> 8192 with the rounding of the input: 270 us alone, 316 us back to back (980 W, 1.55 GHz; 8 row tiles walked
+ * together instead of 16: 321 us); copies and MMAs without
+ * the sums 207 us.  Measured on the way there (back to back): factors read by the summing warps themselves 341 us (the instructions
+ * that ran once in four blocks stalled each time, those of a loop unrolled by two or four missed the instruction cache: 384 us),
+ * scalar FMAs 337 us, one issuing warp 328 us, sixteen summing warps 409 us; a cluster-scope release on the hand-back (a memory
+ * barrier) and registers copied after a separate wait cost 100 us and more each.
  */
 struct PairCfg {
     static constexpr int STAGE_BYTES = 2 * FP8_BLOCK_BYTES;
     static constexpr int STAGES = 6;
-    static constexpr int STG_PITCH = 33;                        /* floats per row of a warp's 32 x 32 transposing stage */
-    static constexpr int SMEM = 1024 + STAGES * STAGE_BYTES + 8 * 32 * STG_PITCH * 4 + 256;
-    static constexpr int GROUP = 8;                             /* row tiles that are walked together before the next outputs */
+    static constexpr int RING = 8;                              /* blocks whose factors are kept: STAGES + 2, see there */
+    static constexpr int SMEM = 1024 + STAGES * STAGE_BYTES + 8 * 32 * 16 * 4 + RING * 256 * 4 + 256;
+    static constexpr int GROUP = 16;                             /* row tiles that are walked together before the next outputs */
 };
 
 __device__ __forceinline__ void umma_f8_pair(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate)
@@ -466,7 +508,8 @@ k_fp8_pair(const __grid_constant__ CUtensorMap mapW, const __grid_constant__ CUt
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     char *gen = smem_raw + (base - smem_u32(smem_raw));
     float *stage_out = reinterpret_cast<float *>(gen + C::STAGES * C::STAGE_BYTES);
-    char *tail = reinterpret_cast<char *>(stage_out + 8 * 32 * C::STG_PITCH);
+    float *ring = stage_out + 8 * 32 * 16;          /* sx * sw [RING][weight block][128 rows] */
+    char *tail = reinterpret_cast<char *>(ring + C::RING * 256);
     const uint32_t bars = smem_u32(tail);
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(tail + 8 * (2 * C::STAGES + 10));
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
@@ -480,7 +523,7 @@ k_fp8_pair(const __grid_constant__ CUtensorMap mapW, const __grid_constant__ CUt
     const bool leader = rank == 0;
 
     if (threadIdx.x == 0) {
-        for (int s = 0; s < C::STAGES; s++) { mbar_init(full_bar(s), 1); mbar_init(empty_bar(s), 2); }
+        for (int s = 0; s < C::STAGES; s++) { mbar_init(full_bar(s), 3); mbar_init(empty_bar(s), 2); }
         for (int a = 0; a < 4; a++) { mbar_init(tfull_bar(a), 1); mbar_init(tempty_bar(a), 8); }
         for (int h = 0; h < 2; h++) mbar_init(drain_bar + 8u * h, 1);
         *abort_flag = 0;
@@ -587,13 +630,59 @@ k_fp8_pair(const __grid_constant__ CUtensorMap mapW, const __grid_constant__ CUt
                 const long long t0 = clock64();
                 while (!mbar_try(drain_bar + 8u * h, 0) && clock64() - t0 < WAIT_CYCLES) { }
             }
+        } else if (warp == 3) {
+            /* The factors of a block, for the summing warps: on the leader's barrier of the block's stage like its operands, so that the
+               accumulator is there only after them.  A ring's slot is free when the stage is: its MMAs waited for the accumulator
+               of two blocks before, which was read after the factors. */
+            const uint32_t leader_full = leader_addr(full_bar(0));
+            int stage = 0, slot = 0;
+            uint32_t phase = 0;
+            bool ok = true;
+            drk_dep_wait();
+            for (int t = pair; t < tiles && ok; t += pairs) {
+                int mt, nt;
+                place(t, mt, nt);
+                const int last = p.kb - 1;
+                const float *sw0 = p.scales + (size_t)(2 * nt) * p.kb, *sw1 = sw0 + (2 * nt + 1 < p.ob ? p.kb : 0);
+                const float *sx[4];
+#pragma unroll
+                for (int q = 0; q < 4; q++) sx[q] = p.sx + min(mt * 256 + rank * 128 + q * 32 + lane, p.n - 1);
+                float x[2][4], w0[2], w1[2];
+#pragma unroll
+                for (int u = 0; u < 2; u++) {
+                    const int b = min(u, last);
+#pragma unroll
+                    for (int q = 0; q < 4; q++) x[u][q] = ld_ahead(sx[q] + (size_t)b * p.n);
+                    w0[u] = ld_const(sw0 + b);
+                    w1[u] = ld_const(sw1 + b);
+                }
+                for (int b4 = 0; b4 < p.kb && ok; b4 += 2)
+#pragma unroll
+                    for (int u = 0; u < 2; u++) {
+                        if (b4 + u >= p.kb) break;
+                        if (!mbar_wait_warp_inline(empty_bar(stage), phase ^ 1u, abort_flag, p.status, 45)) { ok = false; break; }
+                        float *f = ring + slot * 256 + lane;
+#pragma unroll
+                        for (int q = 0; q < 4; q++) { f[q * 32] = x[u][q] * w0[u]; f[128 + q * 32] = x[u][q] * w1[u]; }
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive_cluster(leader_full + 8u * stage);
+                        const int b = min(b4 + u + 2, last);
+#pragma unroll
+                        for (int q = 0; q < 4; q++) x[u][q] = ld_ahead(sx[q] + (size_t)b * p.n);
+                        w0[u] = ld_const(sw0 + b);
+                        w1[u] = ld_const(sw1 + b);
+                        if (++stage == C::STAGES) { stage = 0; phase ^= 1u; }
+                        if (++slot == C::RING) slot = 0;
+                    }
+            }
         }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
         const int quarter = warp & 3, half = (warp - 4) >> 2;       /* this warp's rows and its weight block of the tile's two */
         const uint32_t lane_base = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(half * 128);
         const uint32_t tempty0 = leader_addr(tempty_bar(0));
-        float *stg = stage_out + (warp - 4) * 32 * C::STG_PITCH;
+        float *stg = stage_out + (warp - 4) * 32 * 16;
+        const float *factor = ring + half * 128 + quarter * 32 + lane;
         const int osize = p.out_type == DRK_F32 ? 4 : 2;
         const bool vec = (reinterpret_cast<uintptr_t>(p.out) % 16 == 0) && (p.ldo * osize % 16 == 0);
         /* an accumulator is in registers: its slot may be written again */
@@ -603,73 +692,64 @@ k_fp8_pair(const __grid_constant__ CUtensorMap mapW, const __grid_constant__ CUt
             if (lane == 0) mbar_arrive_cluster(tempty0 + 8u * a);
         };
         drk_dep_wait();
-        int slot = 0;
+        int slot = 0, at_ring = 0;
         uint32_t sphase = 0;
         bool ok = true;
         for (int t = pair; t < tiles && ok; t += pairs) {
             int mt, nt;
             place(t, mt, nt);
             const int row0 = mt * 256 + rank * 128 + quarter * 32;
-            const bool live = row0 + lane < p.n;
             const int ot = 2 * nt + half;
-            const float4 *sx = reinterpret_cast<const float4 *>(p.sx + (size_t)(live ? row0 + lane : 0) * p.kbp);
-            const float *sw = p.scales + (size_t)(ot < p.ob ? ot : 0) * p.kb;
-            float acc[128];
+            unsigned long long acc[64];
 #pragma unroll
-            for (int j = 0; j < 128; j++) acc[j] = 0.0f;
-            /* sx of four blocks and of the next four, sw of the next block; the next block's product is made between this one's
-               additions, where its latency costs nothing */
-            float4 now = __ldcg(sx), next = p.kb > 4 ? __ldcg(sx + 1) : now;
-            float s = __ldg(sw + (p.kb > 1)), f = now.x * __ldg(sw);
+            for (int j = 0; j < 64; j++) acc[j] = 0ull;
             uint32_t ready = mbar_test(tfull_bar(2 * half + slot), sphase);
             for (int b = 0; b < p.kb; b++) {
                 const uint32_t at = lane_base + (uint32_t)(slot * 256), a = 2 * half + slot;
                 if (!__all_sync(0xffffffffu, ready) && !mbar_wait_warp_inline(tfull_bar(a), sphase, abort_flag, p.status, 44)) { ok = false; break; }
                 tc_fence_after();
-                float f_next = 0.0f;
+                const float f = factor[at_ring];
+                unsigned long long ff;
+                asm("mov.b64 %0, {%1, %1};" : "=l"(ff) : "f"(f));
+                at_ring = (at_ring + 256) & (C::RING * 256 - 1);
 #pragma unroll
                 for (int c = 0; c < 2; c++) {
                     uint32_t r[64];
                     tmem_ld_wait(at + 64u * c, r);
                     if (c == 1) {
                         release(a);
-                        const int b1 = b + 1;
-                        if ((b1 & 3) == 0) {
-                            now = next;
-                            if (b1 + 4 < p.kb) next = __ldcg(sx + b1 / 4 + 1);
-                        }
-                        f_next = ((b1 & 2) ? ((b1 & 1) ? now.w : now.z) : ((b1 & 1) ? now.y : now.x)) * s;
-                        if (b + 2 < p.kb) s = __ldg(sw + b + 2);
                         slot ^= 1;
                         if (!slot) sphase ^= 1u;
                         ready = mbar_test(tfull_bar(2 * half + slot), sphase);
                     }
 #pragma unroll
-                    for (int j = 0; j < 64; j++) acc[64 * c + j] = fmaf(f, __uint_as_float(r[j]), acc[64 * c + j]);
+                    for (int j = 0; j < 64; j += 2) ffma2(acc[32 * c + j / 2], ff, r[j], r[j + 1]);
                 }
-                f = f_next;
             }
             if (!ok) break;
-            /* 32 x 32 at a time through shared memory: a row's 32 outputs are then stored by eight lanes side by side */
-            const int cl = (lane & 7) * 4;
+            /* 32 rows x 16 outputs at a time through shared memory, columns turned by the row: four lanes then store a row's run */
+            const int cl = (lane & 3) * 4;
 #pragma unroll
-            for (int c0 = 0; c0 < 128; c0 += 32) {
+            for (int c0 = 0; c0 < 128; c0 += 16) {
                 __syncwarp();
 #pragma unroll
-                for (int j = 0; j < 32; j++) stg[lane * C::STG_PITCH + j] = acc[c0 + j];
+                for (int j = 0; j < 16; j++) {
+                    const unsigned long long two = acc[(c0 + j) / 2];
+                    stg[lane * 16 + ((j + lane) & 15)] = __uint_as_float((uint32_t)(j & 1 ? two >> 32 : two));
+                }
                 __syncwarp();
                 const int o = ot * FP8_BLOCK + c0 + cl;
                 float bias[4];
 #pragma unroll
                 for (int e = 0; e < 4; e++) bias[e] = p.bias && o + e < p.Nout ? __ldg(p.bias + o + e) : 0.0f;
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    const int rr = i * 4 + (lane >> 3);
+                for (int i = 0; i < 4; i++) {
+                    const int rr = i * 8 + (lane >> 2);
                     const size_t r = (size_t)row0 + rr;
                     if (r >= (size_t)p.n) continue;
                     float v[4];
 #pragma unroll
-                    for (int e = 0; e < 4; e++) v[e] = fp8_act(stg[rr * C::STG_PITCH + cl + e] + bias[e], p.act);
+                    for (int e = 0; e < 4; e++) v[e] = fp8_act(stg[rr * 16 + ((cl + e + rr) & 15)] + bias[e], p.act);
                     const size_t at = r * p.ldo + o;
                     if (vec && o + 4 <= p.Nout) {
                         if (p.out_type == DRK_F32) *reinterpret_cast<float4 *>(static_cast<float *>(p.out) + at) = make_float4(v[0], v[1], v[2], v[3]);
@@ -726,22 +806,26 @@ int drk_fp8_tensor_plan(Fp8Tensor *t, const Fp8Params *p, const void *codes, con
     t->split = 1;
     while (t->split < 8 && tiles * t->split * 2 <= room && t->split * 4 <= p->kb) t->split *= 2;
     t->stages = (p->kb + t->split - 1) / t->split;
-    /* Above 64 rows a block of 128 inputs takes a CTA of k_fp8_swap<128> 0.62 us and a pair of k_fp8_pair, on four times the tile,
-       0.49 us, and the pair starts 1 us later (4096 -> 4096: 256 rows 21 against 26 us, 384 rows 32 against 27 us; 8192 -> 8192,
-       256 rows: 50 against 42 us).  Rounds times blocks decide. */
+    /* Above 64 rows a block of 128 inputs takes a CTA of k_fp8_swap<128> 0.6 us and a pair of k_fp8_pair, on four times the tile,
+       0.4 us, and the pair starts 1 us later (4096 -> 4096: 256 rows 20 against 26 us, 384 rows 32 against 26 us; 8192 -> 8192,
+       256 rows: 50 against 37 us).  Rounds times blocks decide. */
     t->mtiles = (p->n + 255) / 256;
     t->ntiles = (p->ob + 1) / 2;
     const long long ptiles = (long long)t->mtiles * t->ntiles, rounds = ((long long)tiles * t->split + sms - 1) / sms, prounds = (ptiles + sms / 2 - 1) / (sms / 2);
-    t->pairs = p->n > 64 && 4 * prounds * p->kb + 8 <= 5 * rounds * t->stages ? (int)(ptiles < sms / 2 ? ptiles : sms / 2) : 0;
-    t->fuse = !t->pairs && p->n <= FUSE_ROWS;
+    t->pairs = p->n > 64 && 2 * prounds * p->kb + 5 <= 3 * rounds * t->stages ? (int)(ptiles < sms / 2 ? ptiles : sms / 2) : 0;
+    /* rounding inside the product's kernel costs nothing while its four warps keep up with the weights: 16-bit rows, one row, or a
+       short share (25088 -> 4096, fp32: one row 19.8 against 22.2 us, two rows 23.8 against 22.4; 4096 -> 4096, four rows 7.6
+       against 8.2) */
+    t->fuse = !t->pairs && p->n <= FUSE_ROWS && (p->in_type != DRK_F32 || p->n == 1 || p->n * t->stages <= 64);
     /* the attribute holds for the current device, which is the plan's */
     const cudaFuncAttribute dyn = cudaFuncAttributeMaxDynamicSharedMemorySize;
     const cudaError_t e = t->pairs      ? cudaFuncSetAttribute(k_fp8_pair, dyn, PairCfg::SMEM)
-                          : t->fuse     ? cudaFuncSetAttribute(k_fp8_swap<16, true>, dyn, SwapCfg<16, true>::smem(SwapCfg<16, true>::STAGES))
-                          : t->nt == 16 ? cudaFuncSetAttribute(k_fp8_swap<16, false>, dyn, SwapCfg<16, false>::smem(SwapCfg<16, false>::STAGES))
-                          : t->nt == 32 ? cudaFuncSetAttribute(k_fp8_swap<32, false>, dyn, SwapCfg<32, false>::smem(SwapCfg<32, false>::STAGES))
-                          : t->nt == 64 ? cudaFuncSetAttribute(k_fp8_swap<64, false>, dyn, SwapCfg<64, false>::smem(SwapCfg<64, false>::STAGES))
-                                        : cudaFuncSetAttribute(k_fp8_swap<128, false>, dyn, SwapCfg<128, false>::smem(SwapCfg<128, false>::STAGES));
+                          : t->fuse     ? (p->in_type == DRK_F32 ? cudaFuncSetAttribute(k_fp8_swap<16, 4>, dyn, SwapCfg<16, 4>::smem(SwapCfg<16, 4>::STAGES))
+                                                                 : cudaFuncSetAttribute(k_fp8_swap<16, 2>, dyn, SwapCfg<16, 2>::smem(SwapCfg<16, 2>::STAGES)))
+                          : t->nt == 16 ? cudaFuncSetAttribute(k_fp8_swap<16, 0>, dyn, SwapCfg<16, 0>::smem(SwapCfg<16, 0>::STAGES))
+                          : t->nt == 32 ? cudaFuncSetAttribute(k_fp8_swap<32, 0>, dyn, SwapCfg<32, 0>::smem(SwapCfg<32, 0>::STAGES))
+                          : t->nt == 64 ? cudaFuncSetAttribute(k_fp8_swap<64, 0>, dyn, SwapCfg<64, 0>::smem(SwapCfg<64, 0>::STAGES))
+                                        : cudaFuncSetAttribute(k_fp8_swap<128, 0>, dyn, SwapCfg<128, 0>::smem(SwapCfg<128, 0>::STAGES));
     if (e != cudaSuccess) return -1;
     if (encode_rows(&t->mapW, codes, (size_t)p->ob * p->kb * FP8_BLOCK, t->pairs ? 64 : FP8_BLOCK)) return -1;
     return encode_rows(&t->mapX, q, (size_t)p->kb * p->n, t->nt);
@@ -766,7 +850,7 @@ static int cluster_launch(void (*kernel)(KArgs...), unsigned grid, unsigned bloc
     return drk_launched(cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...));
 }
 
-template <int NT, bool FUSE> static int swap_launch(cudaStream_t st, const Fp8Tensor *t, const Fp8Params *p)
+template <int NT, int FUSE> static int swap_launch(cudaStream_t st, const Fp8Tensor *t, const Fp8Params *p)
 {
     using C = SwapCfg<NT, FUSE>;
     const int stages = t->stages > C::STAGES ? C::STAGES : t->stages;
@@ -777,9 +861,9 @@ template <int NT, bool FUSE> static int swap_launch(cudaStream_t st, const Fp8Te
 int drk_fp8_tensor_launch(cudaStream_t st, const Fp8Tensor *t, const Fp8Params *p)
 {
     if (t->pairs) return cluster_launch(k_fp8_pair, 2u * t->pairs, 384, 2, PairCfg::SMEM, st, t->mapW, t->mapX, *p, t->mtiles, t->ntiles);
-    if (t->fuse) return swap_launch<16, true>(st, t, p);
-    return t->nt == 16   ? swap_launch<16, false>(st, t, p)
-           : t->nt == 32 ? swap_launch<32, false>(st, t, p)
-           : t->nt == 64 ? swap_launch<64, false>(st, t, p)
-                         : swap_launch<128, false>(st, t, p);
+    if (t->fuse) return (p->in_type == DRK_F32 ? swap_launch<16, 4>(st, t, p) : swap_launch<16, 2>(st, t, p));
+    return t->nt == 16   ? swap_launch<16, 0>(st, t, p)
+           : t->nt == 32 ? swap_launch<32, 0>(st, t, p)
+           : t->nt == 64 ? swap_launch<64, 0>(st, t, p)
+                         : swap_launch<128, 0>(st, t, p);
 }
