@@ -30,10 +30,13 @@
 #define LP_NT 256           /* threads of a CTA, four of which share an SM */
 #define LP_SPLIT 8          /* CTAs that share a row at most */
 #define LP_U 4              /* 16-byte loads a thread has under way, twice (the next batch is requested before this one is used) */
-#define LP_SLOTS 8          /* parts of a thread's share whose maxima are kept */
+#define LP_SLOTS 16         /* parts of a thread's share whose maxima are kept */
 #define LP_GROUPS 64
-#define LP_CAND 2048        /* values and slots that a selection may look at; more: a narrower bound, then one pass per alternative */
-#define LP_ITEMS 2048
+#define LP_CAND 1024        /* values and slots that a selection may look at; more: a narrower bound, then one pass per alternative */
+#define LP_ITEMS 1024
+#define LP_WU 8             /* 16-byte loads of a lane that a warp's row may take: 1024 values in 32 bits, 2048 in 16 */
+#define LP_WNT 128          /* threads of a CTA whose warps have a row each */
+#define LP_WCAND 288        /* values that a warp ranks */
 #define LP_LOW (-200.0f)    /* 2^-200 is zero in 32 bits: exponents are not held below it, so that no 0 * inf appears */
 
 struct LpParams {
@@ -132,6 +135,49 @@ __device__ __forceinline__ int lp_rank(const unsigned long long *keys, int n, un
     return r;
 }
 
+/* S and T of a few values below the maximum m, two at a time; d is held above LP_LOW, NaN too */
+template <bool PACKED> struct LpSums {
+    const float m, c;
+    float s0 = 0.0f, s1 = 0.0f, t0 = 0.0f, t1 = 0.0f;
+    __device__ __forceinline__ LpSums(float m, float c) : m(m), c(c) {}
+    __device__ __forceinline__ void add(float x0, float x1)
+    {
+        const float d0 = fmaxf((x0 - m) * c, LP_LOW), d1 = fmaxf((x1 - m) * c, LP_LOW);
+        const float e0 = lp_exp2(d0), e1 = lp_exp2(d1);
+        s0 += e0; s1 += e1;
+        t0 = fmaf(e0, d0, t0); t1 = fmaf(e1, d1, t1);
+    }
+    __device__ __forceinline__ void join(float &S, float &T) const { S += s0 + s1; T += t0 + t1; }
+};
+/* the same operations on pairs of registers: 2048 x 131072 bf16 106 instead of 110 us; in 32 bits the pairs that the loads leave
+ * cost more than they save (1000 x 32000: 33.6 instead of 30.8 us) */
+template <> struct LpSums<true> {
+    unsigned long long m, c, s = 0, t = 0;
+    __device__ __forceinline__ LpSums(float m_, float c_)
+    {
+        asm("mov.b64 %0, {%1, %1};" : "=l"(m) : "f"(-m_));
+        asm("mov.b64 %0, {%1, %1};" : "=l"(c) : "f"(c_));
+    }
+    __device__ __forceinline__ void add(float x0, float x1)
+    {
+        float d0, d1;
+        asm("{\n\t.reg .b64 x;\n\tmov.b64 x, {%2, %3};\n\tadd.rn.f32x2 x, x, %4;\n\tmul.rn.f32x2 x, x, %5;\n\tmov.b64 {%0, %1}, x;\n\t}"
+            : "=f"(d0), "=f"(d1) : "f"(x0), "f"(x1), "l"(m), "l"(c));
+        d0 = fmaxf(d0, LP_LOW); d1 = fmaxf(d1, LP_LOW);
+        const float e0 = lp_exp2(d0), e1 = lp_exp2(d1);
+        asm("{\n\t.reg .b64 e, d;\n\tmov.b64 e, {%2, %3};\n\tmov.b64 d, {%4, %5};\n\tadd.rn.f32x2 %0, %0, e;\n\tfma.rn.f32x2 %1, e, d, %1;\n\t}"
+            : "+l"(s), "+l"(t) : "f"(e0), "f"(e1), "f"(d0), "f"(d1));
+    }
+    __device__ __forceinline__ void join(float &S, float &T) const
+    {
+        float a, b;
+        asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(s));
+        S += a + b;
+        asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(t));
+        T += a + b;
+    }
+};
+
 /* S and T after the maximum grew by D (in base 2, times the scale) */
 __device__ __forceinline__ void lp_rescale(float D, float &S, float &T)
 {
@@ -140,6 +186,173 @@ __device__ __forceinline__ void lp_rescale(float D, float &S, float &T)
         const float f = lp_exp2(-D);
         T = f * (T - D * S);
         S *= f;
+    }
+}
+
+/* what a row's largest value, its sum and the order of its largest value (NaN included) make of a logit */
+struct LpScore {
+    float M, S, scale, logS;
+    bool none, bad;
+    __device__ __forceinline__ LpScore(const LpParams &p, float M, float S, uint32_t O) :
+        M(M), S(S), scale(p.scale), logS(logf(S)), none(M == -INFINITY && O == lp_order(-INFINITY)), bad(O >= lp_order(INFINITY)) {}
+    __device__ __forceinline__ float operator()(float x) const
+    {
+        return bad ? __uint_as_float(0x7fffffffu) : none || x == -INFINITY ? -INFINITY : (x - M) * scale - logS;
+    }
+    __device__ __forceinline__ float entropy(float E) const { return bad ? __uint_as_float(0x7fffffffu) : none ? 0.0f : logS - E / S * LP_LN2; }
+};
+
+/*
+ * Short rows: a warp holds one in registers, so the maximum is known before the sum and no barrier is needed.  The k-th largest
+ * of the lanes' maxima bounds the k-th largest value; vectors that reach it are read again and ranked as above.
+ */
+template <typename T, int U>
+__global__ void __launch_bounds__(LP_WNT) k_logprobs_short(const LpParams p, const int n)
+{
+    using Y = LpType<T>;
+    constexpr int V = Y::V;
+    __shared__ __align__(16) unsigned long long cands[LP_WNT / 32][LP_WCAND + 2], lists[LP_WNT / 32][LP_KMAX];
+    __shared__ __align__(16) uint32_t lanes[LP_WNT / 32][32];
+    __shared__ uint16_t items[LP_WNT / 32][32 * U];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const size_t row = (size_t)blockIdx.x * (LP_WNT / 32) + warp;
+    drk_dep_wait();
+    drk_dep_trigger();
+    if (row >= (size_t)n) return;
+    const T *v = static_cast<const T *>(p.logits) + row * p.ld;
+    const int head = min(p.len, (int)((16 - (uintptr_t)v % 16) % 16 / sizeof(T)));
+    const int nvec = (p.len - head) / V, singles = p.len - nvec * V;
+    const uint4 *vec = reinterpret_cast<const uint4 *>(v + head);
+    const float c = p.scale * 1.44269504f;
+    const int single = lane < head ? lane : nvec * V + lane;
+    uint4 x[U];
+#pragma unroll
+    for (int u = 0; u < U; u++) x[u] = u * 32 + lane < nvec ? __ldg(vec + u * 32 + lane) : make_uint4(Y::FILL, Y::FILL, Y::FILL, Y::FILL);
+    float alone = lane < singles ? Y::one(v + single) : -INFINITY;
+    int label = -1;
+    float labelled = 0.0f;
+    if (lane < p.m) {
+        label = p.labels[row * p.m + lane];
+        if (label >= 0 && label < p.len) labelled = Y::one(v + label);
+    }
+    unsigned long long *cand = cands[warp], *list = lists[warp];
+    list[lane] = 0;
+
+    float vm[U], mine = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        vm[u] = Y::last(Y::max2(Y::max2(x[u].x, x[u].y), Y::max2(x[u].z, x[u].w)));
+        mine = lp_max_nan(mine, vm[u]);
+    }
+    const uint32_t own = max(lane < nvec ? lp_order(mine) : 0u, lane < singles ? lp_order(alone) : 0u);
+    const uint32_t O = __reduce_max_sync(0xffffffffu, own);
+    float M = fmaxf(mine, alone);           /* the largest that is a number */
+    for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+    float S = 0.0f, E = 0.0f;
+    {
+        const float d = fmaxf((alone - M) * c, LP_LOW), e = lp_exp2(d);
+        S += e;
+        E = fmaf(e, d, E);
+    }
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        float y[V], s = 0.0f, t = 0.0f;
+        Y::unpack(x[u], y);
+#pragma unroll
+        for (int j = 0; j < V; j++) {
+            const float d = fmaxf((y[j] - M) * c, LP_LOW), e = lp_exp2(d);
+            s += e;
+            t = fmaf(e, d, t);
+        }
+        S += s;
+        E += t;
+    }
+    for (int o = 16; o > 0; o >>= 1) { S += __shfl_xor_sync(0xffffffffu, S, o); E += __shfl_xor_sync(0xffffffffu, E, o); }
+
+    if (p.k > 0) {
+        lanes[warp][lane] = own;
+        __syncwarp();
+        int r = 0;
+#pragma unroll
+        for (int j = 0; j < 32; j += 4) {
+            const uint4 y = *reinterpret_cast<const uint4 *>(&lanes[warp][j]);
+            r += (y.x > own || (y.x == own && j < lane)) + (y.y > own || (y.y == own && j + 1 < lane)) + (y.z > own || (y.z == own && j + 2 < lane)) +
+                 (y.w > own || (y.w == own && j + 3 < lane));
+        }
+        const uint32_t border = __shfl_sync(0xffffffffu, own, __ffs(__ballot_sync(0xffffffffu, r == p.k - 1)) - 1);
+        const float low = lp_value(border);         /* NaN where everything counts */
+        const uint32_t before = (1u << lane) - 1;
+        int count = 0, found = 0;
+        auto offer = [&](bool here, float a, int i) {       /* by the whole warp */
+            here = here && !(a < low);
+            const uint32_t all = __ballot_sync(0xffffffffu, here);
+            const int at = count + __popc(all & before);
+            if (here && at < LP_WCAND) cand[at] = lp_key(lp_order(a), (uint32_t)i);
+            count += __popc(all);
+        };
+        if (singles > 0) offer(lane < singles, alone, single);
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const bool here = u * 32 + lane < nvec && !(vm[u] < low);
+            const uint32_t all = __ballot_sync(0xffffffffu, here);
+            if (here) items[warp][found + __popc(all & before)] = (uint16_t)(u * 32 + lane);
+            found += __popc(all);
+        }
+        __syncwarp();
+        for (int w = lane; w - lane < found; w += 32) {
+            const int i = w < found ? items[warp][w] : 0;
+            float y[V];
+            Y::unpack(__ldg(vec + i), y);
+#pragma unroll
+            for (int j = 0; j < V; j++) offer(w < found, y[j], head + i * V + j);
+        }
+        __syncwarp();
+        if (count <= LP_WCAND) {
+            for (int i = lane; i < count; i += 32) {
+                const unsigned long long key = cand[i];
+                const int at = lp_rank(cand, count, key);
+                if (at < p.k) list[at] = key;
+            }
+        } else {
+            /* many values equal to the bound: one pass over the row for each alternative */
+            unsigned long long limit = ~0ull;
+            for (int a = 0; a < p.k; a++) {
+                unsigned long long best = 0;
+                auto look_at = [&](float z, int i) {
+                    const unsigned long long key = lp_key(lp_order(z), (uint32_t)i);
+                    if (key <= limit && key > best) best = key;
+                };
+                if (lane < singles) look_at(alone, single);
+                for (int i = lane; i < nvec; i += 32) {
+                    float y[V];
+                    Y::unpack(__ldg(vec + i), y);
+#pragma unroll
+                    for (int j = 0; j < V; j++) look_at(y[j], head + i * V + j);
+                }
+                for (int o = 16; o > 0; o >>= 1) {
+                    const unsigned long long y = __shfl_xor_sync(0xffffffffu, best, o);
+                    best = y > best ? y : best;
+                }
+                if (lane == 0) list[a] = best;
+                limit = best ? best - 1 : 0;
+            }
+        }
+        __syncwarp();
+    }
+
+    const LpScore score(p, M, S, O);
+    if (p.entropy && lane == 0) p.entropy[row] = score.entropy(E);
+    for (int j = lane; j < p.m; j += 32) {
+        if (j != lane) {
+            label = p.labels[row * p.m + j];
+            if (label >= 0 && label < p.len) labelled = Y::one(v + label);
+        }
+        p.logprob[row * p.m + j] = label < 0 ? 0.0f : label >= p.len ? __uint_as_float(0x7fffffffu) : score(labelled);
+    }
+    if (lane < p.k) {
+        const unsigned long long key = list[lane];
+        p.top_logprob[row * p.k + lane] = score(lp_value((uint32_t)(key >> 32)));
+        p.top_index[row * p.k + lane] = (int)(0xffffffffu - (uint32_t)key);
     }
 }
 
@@ -181,7 +394,9 @@ __global__ void __launch_bounds__(NT, 1024 / NT) k_logprobs(const LpParams p)
     }
 
     float m = -INFINITY, RS = 0.0f, RT = 0.0f, mine = -INFINITY;
-    const int batches = (count + NT * LP_U - 1) / (NT * LP_U), per_slot = max(1, (batches + LP_SLOTS - 1) / LP_SLOTS);
+    const int batches = (count + NT * LP_U - 1) / (NT * LP_U), few = max(1, (batches + 7) / 8);
+    /* parts of up to four batches: eight; longer ones are cut again, as they are read again */
+    const int per_slot = few <= 4 ? few : max(4, (batches + LP_SLOTS - 1) / LP_SLOTS), slots = (batches + per_slot - 1) / per_slot;
     uint4 next[LP_U];
     auto fetch = [&](int b) {
 #pragma unroll
@@ -190,14 +405,21 @@ __global__ void __launch_bounds__(NT, 1024 / NT) k_logprobs(const LpParams p)
             next[u] = i < count ? __ldg(vec + i) : make_uint4(Y::FILL, Y::FILL, Y::FILL, Y::FILL);
         }
     };
+    /* 16-bit rows, whose sums leave a CTA less time for its loads, are also asked into the L2 one batch further ahead */
+    auto ahead = [&](int from, int to) {
+        const int a = from * NT * LP_U, z = min(count, to * NT * LP_U);
+        if (sizeof(T) == 2 && tid == 0 && a < z) asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(vec + a), "r"((z - a) * 16) : "memory");
+    };
+    ahead(1, 2);
     if (batches > 0) fetch(0);
-    for (int slot = 0; slot < LP_SLOTS; slot++) {
+    for (int slot = 0; slot < slots; slot++) {
         float sm = -INFINITY;
         for (int b = slot * per_slot; b < min(batches, (slot + 1) * per_slot); b++) {
             uint4 now[LP_U];
 #pragma unroll
             for (int u = 0; u < LP_U; u++) now[u] = next[u];
             if (b + 1 < batches) fetch(b + 1);
+            ahead(b + 2, b + 3);
             uint32_t w2 = Y::max2(now[0].x, now[0].y);
             w2 = Y::max2(w2, Y::max2(now[0].z, now[0].w));
 #pragma unroll
@@ -209,21 +431,15 @@ __global__ void __launch_bounds__(NT, 1024 / NT) k_logprobs(const LpParams p)
                 m = bm;
             }
             /* a batch is summed by itself: a long row adds len / (threads x 16 or 32) of them, not its values, to one sum */
-            float s0 = 0.0f, s1 = 0.0f, t0 = 0.0f, t1 = 0.0f;
+            LpSums<sizeof(T) == 2> sums(m, c);
 #pragma unroll
             for (int u = 0; u < LP_U; u++) {
                 float x[V];
                 Y::unpack(now[u], x);
 #pragma unroll
-                for (int j = 0; j < V; j += 2) {
-                    const float d0 = fmaxf((x[j] - m) * c, LP_LOW), d1 = fmaxf((x[j + 1] - m) * c, LP_LOW);    /* NaN: LP_LOW too */
-                    const float e0 = lp_exp2(d0), e1 = lp_exp2(d1);
-                    s0 += e0; s1 += e1;
-                    t0 = fmaf(e0, d0, t0); t1 = fmaf(e1, d1, t1);
-                }
+                for (int j = 0; j < V; j += 2) sums.add(x[j], x[j + 1]);
             }
-            RS += s0 + s1;
-            RT += t0 + t1;
+            sums.join(RS, RT);
         }
         smax[slot][tid] = sm;
         mine = lp_max_nan(mine, sm);
@@ -291,7 +507,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) k_logprobs(const LpParams p)
             };
             if (tid < singles) offer(own_single, single_index(tid));
             if (own >= border && own > 0)
-                for (int s = 0; s < LP_SLOTS && s * per_slot < batches; s++)
+                for (int s = 0; s < slots; s++)
                     if (lp_key(lp_order(smax[s][tid]), (uint32_t)(first + (s * per_slot * LP_U * NT + tid) * V)) >= bound) {
                         const int at = atomicAdd(&n_items, 1);
                         if (at < LP_ITEMS) items[at] = (uint32_t)tid | ((uint32_t)s << 16);
@@ -318,7 +534,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) k_logprobs(const LpParams p)
             unsigned long long key = 0;
             if (own > 0) {
                 int s = 0;
-                while (s < LP_SLOTS - 1 && lp_order(smax[s][tid]) != own) s++;
+                while (s < slots - 1 && lp_order(smax[s][tid]) != own) s++;
                 for (int w = 0; w < per_slot * LP_U && key == 0; w++) {
                     const int i = (s * per_slot * LP_U + w) * NT + tid;
                     if (i >= count) break;
@@ -354,7 +570,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) k_logprobs(const LpParams p)
             }
         } else {
             /* the largest values crowd in few threads' shares: one pass over the row for each alternative */
-            unsigned long long last = ~0ull;
+            unsigned long long limit = ~0ull;
             for (int r = 0; r < p.k; r++) {
                 unsigned long long best = 0;
                 for (int i = tid; i < count; i += NT) {
@@ -363,12 +579,12 @@ __global__ void __launch_bounds__(NT, 1024 / NT) k_logprobs(const LpParams p)
 #pragma unroll
                     for (int j = 0; j < V; j++) {
                         const unsigned long long key = lp_key(lp_order(x[j]), (uint32_t)(first + i * V + j));
-                        if (key < last && key > best) best = key;
+                        if (key <= limit && key > best) best = key;
                     }
                 }
                 if (tid < singles) {
                     const unsigned long long key = lp_key(own_single, (uint32_t)single_index(tid));
-                    if (key < last && key > best) best = key;
+                    if (key <= limit && key > best) best = key;
                 }
                 for (int o = 16; o > 0; o >>= 1) {
                     const unsigned long long y = __shfl_xor_sync(0xffffffffu, best, o);
@@ -379,7 +595,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) k_logprobs(const LpParams p)
                 __syncthreads();
                 for (int w = 0; w < WARPS; w++) best = red[w] > best ? red[w] : best;
                 if (tid == 0) list[r] = best;
-                last = best;
+                limit = best ? best - 1 : 0;
             }
         }
     }
@@ -414,22 +630,34 @@ __global__ void __launch_bounds__(NT, 1024 / NT) k_logprobs(const LpParams p)
         __syncthreads();
     }
 
-    const bool none = M == -INFINITY && O == lp_order(-INFINITY), bad = O >= lp_order(INFINITY);
-    const float nan = __uint_as_float(0x7fffffffu), logS = logf(S);
-    auto score = [&](float x) { return bad ? nan : none || x == -INFINITY ? -INFINITY : (x - M) * p.scale - logS; };
-    if (p.entropy && tid == 0) p.entropy[row] = bad ? nan : none ? 0.0f : logS - E / S * LP_LN2;
+    const LpScore score(p, M, S, O);
+    if (p.entropy && tid == 0) p.entropy[row] = score.entropy(E);
     for (int j = tid; j < p.m; j += NT) {
         if (j != tid) {
             label = p.labels[row * p.m + j];
             if (label >= 0 && label < p.len) labelled = Y::one(v + label);
         }
-        p.logprob[row * p.m + j] = label < 0 ? 0.0f : label >= p.len ? nan : score(labelled);
+        p.logprob[row * p.m + j] = label < 0 ? 0.0f : label >= p.len ? __uint_as_float(0x7fffffffu) : score(labelled);
     }
     for (int j = tid; j < p.k; j += NT) {
         const unsigned long long key = list[j];
         p.top_logprob[row * p.k + j] = score(lp_value((uint32_t)(key >> 32)));
         p.top_index[row * p.k + j] = (int)(0xffffffffu - (uint32_t)key);
     }
+}
+
+template <typename T, int U> static int lp_launch_short(cudaStream_t st, const LpParams &p, int n)
+{
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)((n + LP_WNT / 32 - 1) / (LP_WNT / 32)));
+    cfg.blockDim = dim3(LP_WNT);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = drk_dep_launch_enabled() ? 1 : 0;
+    return drk_launched(cudaLaunchKernelEx(&cfg, k_logprobs_short<T, U>, p, n));
 }
 
 static int lp_refuse(const char *why)
@@ -469,10 +697,12 @@ template <typename T, int NT> static int lp_launch(cudaStream_t st, const LpPara
 template <typename T> static int lp_run(cudaStream_t st, LpParams &p, int n)
 {
     constexpr int V = LpType<T>::V;
+    if (p.len <= 32 * LP_WU * V) return lp_launch_short<T, LP_WU>(st, p, n);
+    if (p.len <= 64 * LP_WU * V) return lp_launch_short<T, 2 * LP_WU>(st, p, n);
     const int room = 2 * 148 / n, most = p.len / (LP_NT * V);
     p.split = room < most ? room : most;
     p.split = p.split < 1 ? 1 : p.split > LP_SPLIT ? LP_SPLIT : p.split;
-    return p.len / p.split <= 128 * LP_U * V ? lp_launch<T, 128>(st, p, n) : lp_launch<T, LP_NT>(st, p, n);
+    return n > 4 * 148 || p.len / p.split <= (p.split > 1 ? 2 : 4) * 128 * LP_U * V ? lp_launch<T, 128>(st, p, n) : lp_launch<T, LP_NT>(st, p, n);
 }
 
 extern "C" int dRk_logprobs(dRk_stream stream, const void *logits, int type, long long ld, int n, int len, float scale, const int *labels, int m,

@@ -254,3 +254,53 @@ def test_long_rows_past_32_bits_of_bytes():
     v[-2:] = torch.randn(2, length, device="cuda")
     got = [t[-2:] for t in call(v, None, 4)]
     check(v[-2:], got, None, 4, 1.0)
+
+
+# Rows of up to 8 or 16 vectors a lane are held by a warp: 32 partial sums of at most 16 + 8 + 7 additions, below the len / 128 + 64
+# that check() allows.
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("vectors", [8, 16])
+def test_rows_around_what_a_warp_holds(vectors, dtype):
+    most = 32 * vectors * (4 if dtype == torch.float32 else 8)
+    g = torch.Generator().manual_seed(vectors)
+    for length in (most - 9, most - 1, most, most + 1, most + 9):
+        for n, shift in ((1, 0), (5, 1), (6, 3)):
+            flat = torch.full((n * (length + shift) + shift,), math.nan, dtype=dtype, device="cuda")
+            view = flat[shift:].view(n, length + shift)
+            view[:, :length] = (torch.randn(n, length, generator=g) * 2.5).to(dtype).cuda()
+            labels = torch.randint(-1, length + 1, (n, 40), generator=g, dtype=torch.int32).cuda()
+            v = view[:, :length].contiguous()
+            check(v, call(v, labels, 32, 1.25, ld=length + shift, ptr=view.data_ptr()), labels, 32, 1.25)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("length", [32, 289, 1024, 2048, 4096])
+def test_hard_orders_in_rows_of_a_warp(length, dtype):
+    g = torch.Generator().manual_seed(length)
+    i = torch.arange(length)
+    rows = [torch.full((length,), 1.5), torch.full((length,), -math.inf), torch.full((length,), math.nan), torch.full((length,), math.inf),
+            torch.randint(0, 2, (length,), generator=g).float(), torch.where(torch.randint(0, 2, (length,), generator=g) == 1, 0.0, -0.0),
+            i.float() / 64, -i.float() / 64, torch.where(i % 32 == 5, 8.0, 1.0) + torch.randn(length, generator=g),
+            torch.where((i >= length // 2) & (i < length // 2 + 24), 9.0, 1.0), torch.where(i < 3, 1.0, -math.inf), torch.where(i == length - 1, math.nan, 0.0)]
+    v = torch.stack(rows).to(dtype).cuda()
+    for k in (1, 7, 32):
+        labels = torch.randint(0, length, (len(rows), 2), generator=g, dtype=torch.int32).cuda()
+        check(v, call(v, labels, k), labels, k, 1.0)
+
+
+@pytest.mark.parametrize("kind", ["equal", "ascending", "crowded", "spread"])
+@pytest.mark.parametrize("length", [5000, 33000, 131072])
+def test_hard_orders_in_many_long_rows(length, kind):
+    n, k = 600, 32
+    if kind == "equal":
+        v = torch.full((n, length), 1.5, device="cuda")
+    elif kind == "ascending":
+        v = (torch.arange(length, device="cuda").float() / 64).expand(n, length).contiguous()
+    elif kind == "crowded":         # forty of the largest side by side in each row, elsewhere in each
+        v = torch.randn(n, length, device="cuda")
+        at = torch.randint(0, length - 40, (n, 1), device="cuda") + torch.arange(40, device="cuda")
+        v.scatter_add_(1, at, torch.full(at.shape, 30.0, device="cuda"))
+    else:
+        v = torch.randn(n, length, device="cuda")
+    got = [t[::97] for t in call(v, None, k)]
+    check(v[::97], got, None, k, 1.0)
