@@ -22,9 +22,31 @@ template <> __device__ __forceinline__ float fp8_load(const __nv_bfloat16 *p) { 
 template <> __device__ __forceinline__ float fp8_load(const __half *p) { return __half2float(*p); }
 __device__ __forceinline__ float fp8_decode(unsigned char c) { return __half2float(__half(__nv_cvt_fp8_to_halfraw(c, __NV_E4M3))); }
 
+/* the largest magnitude of eight values, NaN aside, two at a time in 16 bits */
+template <typename T> __device__ __forceinline__ float fp8_largest(const uint4 *raw);
+template <> __device__ __forceinline__ float fp8_largest<float>(const uint4 *raw)
+{
+    const float *v = reinterpret_cast<const float *>(raw);
+    float a = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 8; j++) a = fmaxf(a, fabsf(v[j]));
+    return a;
+}
+__device__ __forceinline__ uint32_t fp8_max2(uint32_t a, uint32_t b, __nv_bfloat16) { uint32_t r; asm("max.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b)); return r; }
+__device__ __forceinline__ uint32_t fp8_max2(uint32_t a, uint32_t b, __half) { uint32_t r; asm("max.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b)); return r; }
+template <typename T> __device__ __forceinline__ float fp8_largest(const uint4 *raw)
+{
+    const uint32_t m = 0x7fff7fffu;
+    const uint32_t r = fp8_max2(fp8_max2(raw->x & m, raw->y & m, T()), fp8_max2(raw->z & m, raw->w & m, T()), T());
+    const T *two = reinterpret_cast<const T *>(&r);
+    return fmaxf(fp8_load(two), fp8_load(two + 1));
+}
+
 /* ------------------------------------------------------------------ activations
- * A half warp owns a block of 128 values of one row, 8 per lane, and asks for U blocks before it rounds the first: bound by HBM
- * (reads sizeof(T), writes one byte a value).  4096 x 8192 bf16 with one block under way: 30 us; U = 4: QUANT_BIG.
+ * A half warp owns a block of 128 values of one row, 8 per lane, and asks for U blocks before it rounds the first; each lane
+ * divides for one of them.  Bound by HBM in 32 bits (reads sizeof(T), writes one byte a value; 4096 x 8192: 27 us, 26 at the copy
+ * rate), in 16 bits by the issue too (22 us, 15 at the copy rate; 24 us with every lane dividing for all and a division for each
+ * block's place).  U = 1: 30 us in 16 bits, U = 4: 22 us, U = 8: 25 us.
  * q: [block][n rows][128], sx: [block][n rows]. */
 template <typename T, int U>
 __global__ void __launch_bounds__(256) k_fp8_quantize_rows(const T *__restrict__ in, size_t ldi, unsigned char *__restrict__ q, float *__restrict__ sx,
@@ -36,49 +58,62 @@ __global__ void __launch_bounds__(256) k_fp8_quantize_rows(const T *__restrict__
     const int sub = threadIdx.x & 15;
     const unsigned total = (unsigned)n * (unsigned)kb, halves = gridDim.x * (blockDim.x / 16);
     /* whole warps stay in the loop: both halves shuffle together */
-    for (unsigned i0 = blockIdx.x * (blockDim.x / 16) + (threadIdx.x >> 5) * 2; i0 < total; i0 += U * halves) {
+    unsigned i0 = blockIdx.x * (blockDim.x / 16) + (threadIdx.x >> 5) * 2;
+    const unsigned first = i0 + ((threadIdx.x >> 4) & 1), drow = halves / (unsigned)kb, dblk = halves - drow * (unsigned)kb;
+    unsigned row = first / (unsigned)kb, blk = first - row * (unsigned)kb;
+    for (; i0 < total; i0 += U * halves) {
         uint4 raw[U][W];
-        unsigned row[U], blk[U];
+        unsigned rows[U], blks[U];
+        float a[U];
 #pragma unroll
         for (int u = 0; u < U; u++) {
-            const unsigned i = i0 + ((threadIdx.x >> 4) & 1) + u * halves;
-            row[u] = i < total ? i / (unsigned)kb : 0xffffffffu;
-            blk[u] = i - row[u] * (unsigned)kb;
+            rows[u] = row; blks[u] = blk;
+            const int k0 = (int)blk * FP8_BLOCK + sub * 8;
+            const T *src = in + row * ldi + k0;
 #pragma unroll
             for (int j = 0; j < W; j++) raw[u][j] = make_uint4(0u, 0u, 0u, 0u);
-            if (row[u] == 0xffffffffu) continue;
-            const int k0 = (int)blk[u] * FP8_BLOCK + sub * 8;
-            const T *src = in + row[u] * ldi + k0;
-            if (vec && k0 + 8 <= Nin) {
+            if (row < (unsigned)n) {
+                if (vec && k0 + 8 <= Nin) {
 #pragma unroll
-                for (int j = 0; j < W; j++) raw[u][j] = __ldg(reinterpret_cast<const uint4 *>(src) + j);
-            } else {
-                T *one = reinterpret_cast<T *>(raw[u]);
+                    for (int j = 0; j < W; j++) raw[u][j] = __ldg(reinterpret_cast<const uint4 *>(src) + j);
+                } else {
+                    T *one = reinterpret_cast<T *>(raw[u]);
 #pragma unroll
-                for (int j = 0; j < 8; j++) if (k0 + j < Nin) one[j] = src[j];
+                    for (int j = 0; j < 8; j++) if (k0 + j < Nin) one[j] = src[j];
+                }
             }
+            row += drow;
+            blk += dblk;
+            if (blk >= (unsigned)kb) { blk -= kb; row++; }
         }
 #pragma unroll
+        for (int u = 0; u < U; u++) a[u] = fmaxf(FP8_FLOOR, fp8_largest<T>(raw[u]));
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1)
+#pragma unroll
+            for (int u = 0; u < U; u++) a[u] = fmaxf(a[u], __shfl_xor_sync(0xffffffffu, a[u], o));
+        /* a lane divides for one of the U blocks */
+        float b = a[0];
+#pragma unroll
+        for (int u = 1; u < U; u++) b = sub % U == u ? a[u] : b;
+        const float bi = __fdiv_rn(FP8_MAX, b), bs = __fdiv_rn(b, FP8_MAX);
+#pragma unroll
         for (int u = 0; u < U; u++) {
-            if (u > 0 && i0 + u * halves >= total) break;       /* the same for the whole warp: i0 is even, and so is halves */
-            float v[8], a = FP8_FLOOR;
-#pragma unroll
-            for (int j = 0; j < 8; j++) v[j] = fp8_load(reinterpret_cast<const T *>(raw[u]) + j);
-#pragma unroll
-            for (int j = 0; j < 8; j++) a = fmaxf(a, fabsf(v[j]));
-#pragma unroll
-            for (int o = 8; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o));
-            const float inv = __fdiv_rn(FP8_MAX, a);
+            const float inv = U == 1 ? bi : __shfl_sync(0xffffffffu, bi, u, 16);
+            float v[8];
             uint32_t c[2];
 #pragma unroll
+            for (int j = 0; j < 8; j++) v[j] = fp8_load(reinterpret_cast<const T *>(raw[u]) + j) * inv;
+#pragma unroll
             for (int j = 0; j < 2; j++) {
-                const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(v[4 * j] * inv, v[4 * j + 1] * inv), __NV_SATFINITE, __NV_E4M3);
-                const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(v[4 * j + 2] * inv, v[4 * j + 3] * inv), __NV_SATFINITE, __NV_E4M3);
+                const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(v[4 * j], v[4 * j + 1]), __NV_SATFINITE, __NV_E4M3);
+                const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(v[4 * j + 2], v[4 * j + 3]), __NV_SATFINITE, __NV_E4M3);
                 c[j] = lo | (hi << 16);
             }
-            if (row[u] != 0xffffffffu) {
-                *reinterpret_cast<uint2 *>(q + ((size_t)blk[u] * n + row[u]) * FP8_BLOCK + sub * 8) = make_uint2(c[0], c[1]);
-                if (sub == 0) sx[(size_t)blk[u] * n + row[u]] = __fdiv_rn(a, FP8_MAX);
+            if (rows[u] < (unsigned)n) {
+                const size_t at = (size_t)blks[u] * n + rows[u];
+                *reinterpret_cast<uint2 *>(q + at * FP8_BLOCK + sub * 8) = make_uint2(c[0], c[1]);
+                if (sub == u) sx[at] = bs;
             }
         }
     }
@@ -279,11 +314,11 @@ extern "C" dRk_Fp8FcPlan *dRk_fp8_fc_plan(const void *in, int in_type, long long
 
 template <typename T> static int fp8_quantize(const dRk_Fp8FcPlan *p, cudaStream_t st)
 {
-    /* few blocks: one for each half warp; many: four under way in each */
+    /* few blocks: one for each half warp; many: two under way in each, eight CTAs to an SM */
     const size_t halves = (size_t)p->p.n * p->p.kb;
     const bool many = halves > 4 * 16 * 148 * 4;
-    const unsigned blocks = drk_blocks(many ? (halves + 3) / 4 : halves, 16, 148u * 16u);
-    return drk_launched(drk_launch_dep(many ? k_fp8_quantize_rows<T, 4> : k_fp8_quantize_rows<T, 1>, dim3(blocks), dim3(256), 0, st, (const T *)p->p.in,
+    const unsigned blocks = drk_blocks(many ? (halves + 1) / 2 : halves, 16, 148u * 8u);
+    return drk_launched(drk_launch_dep(many ? k_fp8_quantize_rows<T, 2> : k_fp8_quantize_rows<T, 1>, dim3(blocks), dim3(256), 0, st, (const T *)p->p.in,
                                        p->p.ldi, p->q, p->sx, p->p.n, p->p.Nin, p->p.kb, p->p.vec));
 }
 

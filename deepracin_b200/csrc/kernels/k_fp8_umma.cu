@@ -151,10 +151,15 @@ __device__ __forceinline__ bool mbar_wait1(uint32_t bar, uint32_t parity, volati
 /*
  * Few rows: the weights are on the M side (a packed block of 128 outputs x 128 inputs per stage, the only large operand), NT
  * rows of the input on the N side.  A cluster of `split` CTAs shares the K blocks of one tile; each sends its sums of a row to
- * the CTA that owns the row (distributed shared memory), which adds them in the order of the ranks.  Warp 0 issues TMA, warp 1 the MMAs; two groups of four warps own the
- * 128 outputs, one per lane, and add the blocks times sx * sw to NT sums each, taking turns (what a block costs them beside the
- * additions -- the wait, the factors -- is 350 of 600 clocks); with NT = 128 each has half of the rows instead.  A block's
- * accumulator is one of SLOTS in TMEM.  The weights do not depend on the launch in front: their first blocks are on the way before it ends.
+ * the CTA that owns the row (distributed shared memory), which adds them in the order of the ranks.  Warp 0 issues TMA, warp 1
+ * the MMAs; two groups of four warps own the 128 outputs, one per lane, and add the blocks times sx * sw to NT sums each, taking
+ * turns (what a block costs them beside the additions -- the wait, the factors -- is 350 of 600 clocks); with NT = 128 each has
+ * half of the rows instead.  A block's accumulator is one of SLOTS in TMEM.  The weights do not depend on the launch in front:
+ * their first blocks are on the way before it ends.
+ *
+ * Bound by the weights' way from HBM behind 4 us of launch, first loads and exchange: 1 x 25088 -> 4096 fp32 19.8 us (15.7 at the
+ * copy rate), 1 x 4096 -> 4096 6.1 us (2.6); with 64 rows by the sums of a block too, and the rounding's launch: 64 x 25088 -> 4096
+ * 25.1 us (16.8), 64 x 4096 -> 1000 8.1 us; with NT = 128 by the sums, 0.6 us a block.
  *
  * FUSE (the bytes of an input value; at most FUSE_ROWS rows): four more warps round the input themselves, a block each in turn,
  * straight into the swizzled operand tile; what takes two launches takes one.
@@ -464,8 +469,7 @@ k_fp8_swap(const __grid_constant__ CUtensorMap mapW, const __grid_constant__ CUt
  * What bounds it: the way issue -> commit -> read -> hand back -> issue, 700 to 900 clocks a block with two accumulators under
  * way, where the MMAs take 512; in a long run the board's power (half of it spent on copies and at rest, a third on the MMAs).
  * 4096 x 8192 -> 8192 with the rounding of the input: 270 us alone, 316 us back to back (980 W, 1.55 GHz; 8 row tiles walked
- * together instead of 16: 321 us); copies and MMAs without
- * the sums 207 us.  Measured on the way there (back to back): factors read by the summing warps themselves 341 us (the instructions
+ * together instead of 16: 321 us); copies and MMAs without the sums 207 us.  Measured on the way there (back to back): factors read by the summing warps themselves 341 us (the instructions
  * that ran once in four blocks stalled each time, those of a loop unrolled by two or four missed the instruction cache: 384 us),
  * scalar FMAs 337 us, one issuing warp 328 us, sixteen summing warps 409 us; a cluster-scope release on the hand-back (a memory
  * barrier) and registers copied after a separate wait cost 100 us and more each.

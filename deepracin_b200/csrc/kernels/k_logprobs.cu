@@ -10,14 +10,17 @@
  * One pass over the row: each thread holds a running maximum, S and T, rescaled when its maximum grows (d falls by D, so
  * S -> 2^-D S and T -> 2^-D (T - D S); exponents are kept in base 2), and writes down the maximum of every slot of its share.
  * The k-th largest of the maxima of 64 groups of threads bounds the k-th largest value from below, so only slots whose maximum
- * reaches it are read again (for 131072 normal logits and k = 20 about 30 of 4096 slots), and what reaches it is ranked by
+ * reaches it are read again (for 131072 normal logits and k = 20 about 30 of 2048 slots), and what reaches it is ranked by
  * counting.  Few rows are split over a cluster of CTAs, which join through distributed shared memory: one launch, no workspace.
+ * A row that fits a warp's registers is taken by one warp (k_logprobs_short).
  *
- * Bound by HBM in 32 bits (2048 x 131072: 163 us without alternatives = 6.6 TB/s, 178 us with five, 184 us with twenty) and by the
- * issue of about eight instructions a value in 16 bits (1024 x 131072 bf16: 56 and 61 us, 41 us at the copy rate); below that by the
- * chain of a launch, one round of loads and the selection's barriers (1 x 1000: 2.7 us, 4.6 us with five; 1 x 131072 bf16: 4.3 and
- * 8.2 us with twenty).  CTAs of 512 threads instead of 256 took 192 us and 35 instead of 24 us for 1000 x 32000: with two of them
- * on an SM half its loads stop during a selection.  d as one FMA, x c - m c, saved nothing and left a row of one value off zero.
+ * Bound by HBM in 32 bits (2048 x 131072: 158 us without alternatives = 6.8 TB/s, 166 us with five, 175 us with twenty); in 16 bits
+ * and in rows of some thousands by what the CTAs of an SM issue and wait for between two rows' loads (2048 x 131072 bf16: 88, 94
+ * and 102 us, 82 us at the copy rate; 4096 x 8192 fp32: 28, 37 and 39 us, 20 us); below that by the chain of a launch, one round
+ * of loads and the selection's barriers (1 x 131072 bf16: 4.3 and 8.0 us with twenty).  CTAs of 512 threads took 192 us for
+ * 2048 x 131072.  Not kept: maxima of parts of four neighbouring threads, 64 contiguous bytes each (3 us saved at k = 5 in rows of
+ * 8192, 2 us lost at k = 20); the second reading in batches of four loads (39.2 instead of 37.3 us for 4096 x 8192); prefetches
+ * into the L2 for 32-bit rows (1 to 3 us slower); d as one FMA, x c - m c, saved nothing and left a row of one value off zero.
  */
 #include <math.h>
 #include <stdio.h>
@@ -204,7 +207,10 @@ struct LpScore {
 
 /*
  * Short rows: a warp holds one in registers, so the maximum is known before the sum and no barrier is needed.  The k-th largest
- * of the lanes' maxima bounds the k-th largest value; vectors that reach it are read again and ranked as above.
+ * of the lanes' maxima bounds the k-th largest value; vectors that reach it are read again and ranked as above, the places of
+ * both found by ballots.  Bound by the issue of a row's instructions, 20000 x 1000 fp32: 15.5 us without alternatives, 25 us with
+ * five, 31 us with twenty (12 us at the copy rate); a CTA of 128 threads a row took 65, 109 and 117 us, its barriers and single
+ * warps' steps a row's whole time.  1 x 1000: 2.0, 3.0 and 3.2 us.
  */
 template <typename T, int U>
 __global__ void __launch_bounds__(LP_WNT) k_logprobs_short(const LpParams p, const int n)
@@ -395,7 +401,8 @@ __global__ void __launch_bounds__(NT, 1024 / NT) k_logprobs(const LpParams p)
 
     float m = -INFINITY, RS = 0.0f, RT = 0.0f, mine = -INFINITY;
     const int batches = (count + NT * LP_U - 1) / (NT * LP_U), few = max(1, (batches + 7) / 8);
-    /* parts of up to four batches: eight; longer ones are cut again, as they are read again */
+    /* slots of up to four batches: eight; longer ones are cut again, as they are read again (2048 x 131072: 177 us with sixteen,
+       187 with eight; 4000 x 8192 bf16: 34 us with eight, 37 with sixteen) */
     const int per_slot = few <= 4 ? few : max(4, (batches + LP_SLOTS - 1) / LP_SLOTS), slots = (batches + per_slot - 1) / per_slot;
     uint4 next[LP_U];
     auto fetch = [&](int b) {
@@ -692,8 +699,13 @@ template <typename T, int NT> static int lp_launch(cudaStream_t st, const LpPara
 
 /* A row is split over up to eight CTAs while that leaves at most two on each of 148 SMs and a load for each thread of a share.
  * Four would fit, but then the next launch finds no place to start in while this one ends: 148 x 32000 bf16 with 20 alternatives
- * takes 7.6 us unsplit, 8.3 us in twos, 12 to 14 us in threes and fours; 100 x 131072 fp32 27, 19, and 18 us.  Shares of at most
- * one batch of 128 threads run with 128. */
+ * takes 7.6 us unsplit, 8.3 us in twos, 12 to 14 us in threes and fours; 100 x 131072 fp32 27, 19, and 18 us.
+ * CTAs of 128 threads, eight on an SM, when the rows do not all find a place in fours of 256 (4096 x 8192 fp32: 39 instead of
+ * 54 us, 1000 x 32000 28 instead of 31; but 592 x 131072, 61 instead of 51), in 16 bits, where more threads than loads are
+ * missing, when they fill six places of eight (131072 bf16: 700 rows 53 instead of 40 us, 1100 rows 59 both, 2000 rows 96 instead
+ * of 98; 32000 f16: 700 rows 21.0 instead of 19.4, 900 rows 22.0 instead of 22.5, 2000 rows 36.6 instead of 40.3); or when a
+ * share is a few of their batches (300 x 8192 fp32: 6.8 instead of 8.7 us; 1 x 131072 bf16 in eight shares of four batches: 9.7
+ * instead of 8.0 us). */
 template <typename T> static int lp_run(cudaStream_t st, LpParams &p, int n)
 {
     constexpr int V = LpType<T>::V;
@@ -702,7 +714,7 @@ template <typename T> static int lp_run(cudaStream_t st, LpParams &p, int n)
     const int room = 2 * 148 / n, most = p.len / (LP_NT * V);
     p.split = room < most ? room : most;
     p.split = p.split < 1 ? 1 : p.split > LP_SPLIT ? LP_SPLIT : p.split;
-    return n > 4 * 148 || p.len / p.split <= (p.split > 1 ? 2 : 4) * 128 * LP_U * V ? lp_launch<T, 128>(st, p, n) : lp_launch<T, LP_NT>(st, p, n);
+    return n > (sizeof(T) == 2 ? 6 : 4) * 148 || p.len / p.split <= (p.split > 1 ? 2 : 4) * 128 * LP_U * V ? lp_launch<T, 128>(st, p, n) : lp_launch<T, LP_NT>(st, p, n);
 }
 
 extern "C" int dRk_logprobs(dRk_stream stream, const void *logits, int type, long long ld, int n, int len, float scale, const int *labels, int m,
