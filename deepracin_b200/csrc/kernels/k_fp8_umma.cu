@@ -449,12 +449,34 @@ k_fp8_swap(const __grid_constant__ CUtensorMap mapW, const __grid_constant__ CUt
     if (warp == 1) tmem_dealloc(tmem_base, C::TMEM_COLS);
     if (split > 1) cluster_wait();
     else __syncthreads();
+    /* four rows at a time: their reads and stores do not wait for one another */
     if (summing && o < p.Nout)
-        for (int q = part; q < own && r0 + q * split + rank < p.n; q += 2) {
-            float sum = 0.0f;
-#pragma unroll 4
-            for (int s = 0; s < sources; s++) sum += inbox[(s * own + q) * FP8_BLOCK + ol];
-            fp8_put(p, (size_t)r0 + q * split + rank, o, sum + bias);
+        for (int q0 = part; q0 < own && r0 + q0 * split + rank < p.n; q0 += 8) {
+            float sum[4];
+#pragma unroll
+            for (int u = 0; u < 4; u++) sum[u] = 0.0f;
+            for (int s = 0; s < sources; s++)
+#pragma unroll
+                for (int u = 0; u < 4; u++) sum[u] += inbox[(s * own + min(q0 + 2 * u, own - 1)) * FP8_BLOCK + ol];
+            size_t at[4];
+            bool here[4];
+#pragma unroll
+            for (int u = 0; u < 4; u++) {
+                const int q = q0 + 2 * u, r = r0 + q * split + rank;
+                here[u] = q < own && r < p.n;
+                at[u] = (size_t)r * p.ldo + o;
+                sum[u] = fp8_act(sum[u] + bias, p.act);
+            }
+            if (p.out_type == DRK_F32) {
+#pragma unroll
+                for (int u = 0; u < 4; u++) if (here[u]) static_cast<float *>(p.out)[at[u]] = sum[u];
+            } else if (p.out_type == DRK_BF16) {
+#pragma unroll
+                for (int u = 0; u < 4; u++) if (here[u]) static_cast<__nv_bfloat16 *>(p.out)[at[u]] = fp8_store<__nv_bfloat16>(sum[u]);
+            } else {
+#pragma unroll
+                for (int u = 0; u < 4; u++) if (here[u]) static_cast<__half *>(p.out)[at[u]] = fp8_store<__half>(sum[u]);
+            }
         }
 }
 
@@ -731,45 +753,72 @@ k_fp8_pair(const __grid_constant__ CUtensorMap mapW, const __grid_constant__ CUt
                 }
             }
             if (!ok) break;
-            /* 32 rows x 16 outputs at a time through shared memory, columns turned by the row: four lanes then store a row's run */
-            const int cl = (lane & 3) * 4;
-#pragma unroll
-            for (int c0 = 0; c0 < 128; c0 += 16) {
-                __syncwarp();
+            /* 32 rows x 16 outputs at a time through shared memory, columns turned by the row: four lanes then store a row's run.
+               A loop, as code that runs once a tile costs its way from the L2. */
+            const int cl = (lane & 3) * 4, o0 = ot * FP8_BLOCK + cl;
+            auto stage16 = [&](auto chunk) {
 #pragma unroll
                 for (int j = 0; j < 16; j++) {
-                    const unsigned long long two = acc[(c0 + j) / 2];
+                    const unsigned long long two = acc[(decltype(chunk)::value * 16 + j) / 2];
                     stg[lane * 16 + ((j + lane) & 15)] = __uint_as_float((uint32_t)(j & 1 ? two >> 32 : two));
                 }
+            };
+            float bias[4], next[4];
+            auto ask = [&](int o) {
+#pragma unroll
+                for (int e = 0; e < 4; e++) next[e] = p.bias && o + e < p.Nout ? __ldg(p.bias + o + e) : 0.0f;
+            };
+            ask(o0);
+#pragma unroll 1
+            for (int c = 0; c < 8; c++) {
+                const int o = o0 + c * 16;
+#pragma unroll
+                for (int e = 0; e < 4; e++) bias[e] = next[e];
+                if (c < 7) ask(o + 16);
                 __syncwarp();
-                const int o = ot * FP8_BLOCK + c0 + cl;
-                float bias[4];
+                switch (c) {
+                case 0: stage16(std::integral_constant<int, 0>{}); break;
+                case 1: stage16(std::integral_constant<int, 1>{}); break;
+                case 2: stage16(std::integral_constant<int, 2>{}); break;
+                case 3: stage16(std::integral_constant<int, 3>{}); break;
+                case 4: stage16(std::integral_constant<int, 4>{}); break;
+                case 5: stage16(std::integral_constant<int, 5>{}); break;
+                case 6: stage16(std::integral_constant<int, 6>{}); break;
+                default: stage16(std::integral_constant<int, 7>{}); break;
+                }
+                __syncwarp();
+                float v[4][4];
 #pragma unroll
-                for (int e = 0; e < 4; e++) bias[e] = p.bias && o + e < p.Nout ? __ldg(p.bias + o + e) : 0.0f;
+                for (int i = 0; i < 4; i++)
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const int rr = i * 8 + (lane >> 2);
-                    const size_t r = (size_t)row0 + rr;
-                    if (r >= (size_t)p.n) continue;
-                    float v[4];
+                    for (int e = 0; e < 4; e++) {
+                        const int rr = i * 8 + (lane >> 2);
+                        v[i][e] = fp8_act(stg[rr * 16 + ((cl + e + rr) & 15)] + bias[e], p.act);
+                    }
+                const int left = p.n - row0 - (lane >> 2);      /* rows i * 8 below it exist */
+                const size_t at0 = (size_t)(row0 + (lane >> 2)) * p.ldo + o;
+                if (!vec || o + 4 > p.Nout) {
+#pragma unroll 1
+                    for (int e = 0; e < 4 && o + e < p.Nout; e++)
 #pragma unroll
-                    for (int e = 0; e < 4; e++) v[e] = fp8_act(stg[rr * 16 + ((cl + e + rr) & 15)] + bias[e], p.act);
-                    const size_t at = r * p.ldo + o;
-                    if (vec && o + 4 <= p.Nout) {
-                        if (p.out_type == DRK_F32) *reinterpret_cast<float4 *>(static_cast<float *>(p.out) + at) = make_float4(v[0], v[1], v[2], v[3]);
-                        else {
-                            uint2 w;
-                            if (p.out_type == DRK_BF16) {
-                                const __nv_bfloat162 lo = __floats2bfloat162_rn(v[0], v[1]), hi = __floats2bfloat162_rn(v[2], v[3]);
-                                w = make_uint2(*reinterpret_cast<const uint32_t *>(&lo), *reinterpret_cast<const uint32_t *>(&hi));
-                            } else {
-                                const __half2 lo = __floats2half2_rn(v[0], v[1]), hi = __floats2half2_rn(v[2], v[3]);
-                                w = make_uint2(*reinterpret_cast<const uint32_t *>(&lo), *reinterpret_cast<const uint32_t *>(&hi));
-                            }
-                            *reinterpret_cast<uint2 *>(static_cast<char *>(p.out) + at * 2) = w;
+                        for (int i = 0; i < 4; i++)
+                            if (i * 8 < left) fp8_put(p, (size_t)row0 + i * 8 + (lane >> 2), o + e, e == 0 ? v[i][0] : e == 1 ? v[i][1] : e == 2 ? v[i][2] : v[i][3]);
+                } else if (p.out_type == DRK_F32) {
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+                        if (i * 8 < left) *reinterpret_cast<float4 *>(static_cast<float *>(p.out) + at0 + (size_t)(i * 8) * p.ldo) = make_float4(v[i][0], v[i][1], v[i][2], v[i][3]);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        uint2 w;
+                        if (p.out_type == DRK_BF16) {
+                            const __nv_bfloat162 lo = __floats2bfloat162_rn(v[i][0], v[i][1]), hi = __floats2bfloat162_rn(v[i][2], v[i][3]);
+                            w = make_uint2(*reinterpret_cast<const uint32_t *>(&lo), *reinterpret_cast<const uint32_t *>(&hi));
+                        } else {
+                            const __half2 lo = __floats2half2_rn(v[i][0], v[i][1]), hi = __floats2half2_rn(v[i][2], v[i][3]);
+                            w = make_uint2(*reinterpret_cast<const uint32_t *>(&lo), *reinterpret_cast<const uint32_t *>(&hi));
                         }
-                    } else {
-                        for (int e = 0; e < 4 && o + e < p.Nout; e++) fp8_put(p, r, o + e, v[e]);
+                        if (i * 8 < left) *reinterpret_cast<uint2 *>(static_cast<char *>(p.out) + (at0 + (size_t)(i * 8) * p.ldo) * 2) = w;
                     }
                 }
             }
