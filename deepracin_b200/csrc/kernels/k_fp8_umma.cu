@@ -753,15 +753,14 @@ k_fp8_pair(const __grid_constant__ CUtensorMap mapW, const __grid_constant__ CUt
                 }
             }
             if (!ok) break;
-            /* 32 rows x 16 outputs at a time through shared memory, columns turned by the row: four lanes then store a row's run.
-               A loop, as code that runs once a tile costs its way from the L2. */
+            /* 32 rows x 16 outputs at a time through shared memory, the eight pairs of a row exchanged by its number so that
+               neither side meets a bank twice; four lanes then store a row's run.  A loop, as code that runs once a tile costs its
+               way from the L2. */
             const int cl = (lane & 3) * 4, o0 = ot * FP8_BLOCK + cl;
             auto stage16 = [&](auto chunk) {
 #pragma unroll
-                for (int j = 0; j < 16; j++) {
-                    const unsigned long long two = acc[(decltype(chunk)::value * 16 + j) / 2];
-                    stg[lane * 16 + ((j + lane) & 15)] = __uint_as_float((uint32_t)(j & 1 ? two >> 32 : two));
-                }
+                for (int j = 0; j < 8; j++)
+                    reinterpret_cast<unsigned long long *>(stg)[lane * 8 + (j ^ (lane >> 1 & 7))] = acc[decltype(chunk)::value * 8 + j];
             };
             float bias[4], next[4];
             auto ask = [&](int o) {
@@ -789,12 +788,13 @@ k_fp8_pair(const __grid_constant__ CUtensorMap mapW, const __grid_constant__ CUt
                 __syncwarp();
                 float v[4][4];
 #pragma unroll
-                for (int i = 0; i < 4; i++)
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        const int rr = i * 8 + (lane >> 2);
-                        v[i][e] = fp8_act(stg[rr * 16 + ((cl + e + rr) & 15)] + bias[e], p.act);
-                    }
+                for (int i = 0; i < 4; i++) {
+                    const int rr = i * 8 + (lane >> 2);
+                    float4 w = reinterpret_cast<const float4 *>(stg)[rr * 4 + ((lane & 3) ^ (rr >> 2 & 3))];
+                    if (rr >> 1 & 1) w = make_float4(w.z, w.w, w.x, w.y);
+                    v[i][0] = fp8_act(w.x + bias[0], p.act); v[i][1] = fp8_act(w.y + bias[1], p.act);
+                    v[i][2] = fp8_act(w.z + bias[2], p.act); v[i][3] = fp8_act(w.w + bias[3], p.act);
+                }
                 const int left = p.n - row0 - (lane >> 2);      /* rows i * 8 below it exist */
                 const size_t at0 = (size_t)(row0 + (lane >> 2)) * p.ldo + o;
                 if (!vec || o + 4 > p.Nout) {
