@@ -19,7 +19,12 @@ template <> __device__ __forceinline__ __nv_bfloat16 fp8_store<__nv_bfloat16>(fl
 template <> __device__ __forceinline__ __half fp8_store<__half>(float v) { return __float2half_rn(v); }
 
 /* ReLU that lets NaN pass (a comparison with NaN is false) */
-__device__ __forceinline__ float fp8_act(float v, int act) { return act && v < 0.0f ? 0.0f : v; }
+__device__ __forceinline__ float fp8_act(float v, int act)
+{
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(v), "f"(act ? 0.0f : -INFINITY));
+    return r;
+}
 
 struct Fp8Params {
     const void *in;

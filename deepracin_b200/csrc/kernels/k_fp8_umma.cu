@@ -107,9 +107,15 @@ __device__ __forceinline__ void cluster_wait()
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 /* a store to this address in the shared memory of the cluster's CTA `rank` */
-__device__ __forceinline__ void st_cluster(uint32_t saddr, uint32_t rank, float v)
+__device__ __forceinline__ uint32_t cluster_addr(uint32_t saddr, uint32_t rank)
 {
-    asm volatile("{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %0, %1;\n\tst.shared::cluster.f32 [a], %2;\n\t}" ::"r"(saddr), "r"(rank), "f"(v) : "memory");
+    uint32_t a;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(saddr), "r"(rank));
+    return a;
+}
+__device__ __forceinline__ void st_cluster(uint32_t cluster_addr, float v)
+{
+    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(cluster_addr), "f"(v) : "memory");
 }
 __device__ __forceinline__ void fp8_put(const Fp8Params &p, size_t r, int o, float v)
 {
@@ -430,18 +436,39 @@ k_fp8_swap(const __grid_constant__ CUtensorMap mapW, const __grid_constant__ CUt
     tc_fence_before();
     __syncthreads();
     if (split > 1) cluster_wait();
-    /* row j of the tile belongs to CTA j % split, a power of two; inbox [source][row / split][128 outputs] */
+    /* row j of the tile belongs to CTA j % split, a power of two of up to eight; inbox [source][row / split][128 outputs] */
     const bool summing = warp >= 2 && warp < 10;
     const int part = (warp - 2) >> 2, ol = (warp & 3) * 32 + lane, o = ot * FP8_BLOCK + ol;
     const int c0 = C::GROUPS == 2 ? 0 : part * C::COLS, lg = 31 - __clz(split), own = NT >> lg, sources = C::GROUPS * split;
     const float bias = summing && p.bias && o < p.Nout ? __ldg(p.bias + o) : 0.0f;
-    if (summing) {
-        const uint32_t to = smem_u32(inbox + (C::GROUPS * rank + (C::GROUPS == 2 ? part : 0)) * own * FP8_BLOCK + ol);
+    /* one source: its sums are the result */
+    const bool alone = C::GROUPS == 1 && split == 1;
+    if (summing && alone && o < p.Nout) {
+        auto put = [&](auto *out) {
+            out += (size_t)(r0 + c0) * p.ldo + o;
+            const int left = p.n - r0 - c0;
 #pragma unroll
-        for (int j = 0; j < C::COLS; j++) {
-            const int r = c0 + j;
-            if (r0 + r >= p.n) break;
-            st_cluster(to + (uint32_t)(r >> lg) * (FP8_BLOCK * 4), (uint32_t)(r & (split - 1)), acc[j]);
+            for (int j = 0; j < C::COLS; j++) {
+                if (j < left) *out = fp8_store<std::remove_pointer_t<decltype(out)>>(fp8_act(acc[j] + bias, p.act));
+                out += p.ldo;
+            }
+        };
+        if (p.out_type == DRK_F32) put(static_cast<float *>(p.out));
+        else if (p.out_type == DRK_BF16) put(static_cast<__nv_bfloat16 *>(p.out));
+        else put(static_cast<__half *>(p.out));
+    }
+    if (summing && !alone) {
+        const uint32_t to = smem_u32(inbox + (C::GROUPS * rank + (C::GROUPS == 2 ? part : 0)) * own * FP8_BLOCK + ol);
+        /* eight addresses that move on together: what runs once is paid by its length */
+        uint32_t at[8];
+#pragma unroll
+        for (int k = 0; k < 8; k++) at[k] = cluster_addr(to + (uint32_t)((c0 + k) >> lg) * (FP8_BLOCK * 4), (uint32_t)(k & (split - 1)));
+        const uint32_t step = (uint32_t)(8 >> lg) * (FP8_BLOCK * 4);
+#pragma unroll
+        for (int j0 = 0; j0 < C::COLS; j0 += 8) {
+            if (r0 + c0 + j0 >= p.n) break;
+#pragma unroll
+            for (int k = 0; k < 8; k++) { st_cluster(at[k], acc[j0 + k]); at[k] += step; }
         }
     }
     __syncwarp();
@@ -450,7 +477,7 @@ k_fp8_swap(const __grid_constant__ CUtensorMap mapW, const __grid_constant__ CUt
     if (split > 1) cluster_wait();
     else __syncthreads();
     /* four rows at a time: their reads and stores do not wait for one another */
-    if (summing && o < p.Nout)
+    if (summing && !alone && o < p.Nout)
         for (int q0 = part; q0 < own && r0 + q0 * split + rank < p.n; q0 += 8) {
             float sum[4];
 #pragma unroll
