@@ -17,6 +17,9 @@ template <typename T> __device__ __forceinline__ T fp8_store(float v);
 template <> __device__ __forceinline__ float fp8_store<float>(float v) { return v; }
 template <> __device__ __forceinline__ __nv_bfloat16 fp8_store<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 template <> __device__ __forceinline__ __half fp8_store<__half>(float v) { return __float2half_rn(v); }
+template <typename W> __device__ __forceinline__ W fp8_store2(float a, float b);
+template <> __device__ __forceinline__ __nv_bfloat162 fp8_store2<__nv_bfloat162>(float a, float b) { return __floats2bfloat162_rn(a, b); }
+template <> __device__ __forceinline__ __half2 fp8_store2<__half2>(float a, float b) { return __floats2half2_rn(a, b); }
 
 /* ReLU that lets NaN pass (a comparison with NaN is false) */
 __device__ __forceinline__ float fp8_act(float v, int act)

@@ -527,7 +527,7 @@ struct PairCfg {
     static constexpr int STAGE_BYTES = 2 * FP8_BLOCK_BYTES;
     static constexpr int STAGES = 6;
     static constexpr int RING = 8;                              /* blocks whose factors are kept: STAGES + 2, see there */
-    static constexpr int SMEM = 1024 + STAGES * STAGE_BYTES + 8 * 32 * 16 * 4 + RING * 256 * 4 + 256;
+    static constexpr int SMEM = 1024 + STAGES * STAGE_BYTES + 8 * 32 * 16 * 4 + RING * 256 * 4 + 8 * FP8_BLOCK * 4 + 256;
     static constexpr int GROUP = 16;                             /* row tiles that are walked together before the next outputs */
 };
 
@@ -562,7 +562,8 @@ k_fp8_pair(const __grid_constant__ CUtensorMap mapW, const __grid_constant__ CUt
     char *gen = smem_raw + (base - smem_u32(smem_raw));
     float *stage_out = reinterpret_cast<float *>(gen + C::STAGES * C::STAGE_BYTES);
     float *ring = stage_out + 8 * 32 * 16;          /* sx * sw [RING][weight block][128 rows] */
-    char *tail = reinterpret_cast<char *>(ring + C::RING * 256);
+    float *bias_of = ring + C::RING * 256;          /* [summing warp][128 outputs] */
+    char *tail = reinterpret_cast<char *>(bias_of + 8 * FP8_BLOCK);
     const uint32_t bars = smem_u32(tail);
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(tail + 8 * (2 * C::STAGES + 10));
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
@@ -735,6 +736,7 @@ k_fp8_pair(const __grid_constant__ CUtensorMap mapW, const __grid_constant__ CUt
         const uint32_t lane_base = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(half * 128);
         const uint32_t tempty0 = leader_addr(tempty_bar(0));
         float *stg = stage_out + (warp - 4) * 32 * 16;
+        float4 *bias128 = reinterpret_cast<float4 *>(bias_of + (warp - 4) * FP8_BLOCK);
         const float *factor = ring + half * 128 + quarter * 32 + lane;
         const int osize = p.out_type == DRK_F32 ? 4 : 2;
         const bool vec = (reinterpret_cast<uintptr_t>(p.out) % 16 == 0) && (p.ldo * osize % 16 == 0);
@@ -744,6 +746,17 @@ k_fp8_pair(const __grid_constant__ CUtensorMap mapW, const __grid_constant__ CUt
             __syncwarp();
             if (lane == 0) mbar_arrive_cluster(tempty0 + 8u * a);
         };
+        /* this lane's four of the bias of a tile's outputs: asked for while the tile in front is written */
+        auto bias4 = [&](int t) {
+            int mt, nt;
+            place(t, mt, nt);
+            const int o = (2 * nt + half) * FP8_BLOCK + lane * 4;
+            float b[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) b[e] = p.bias && o + e < p.Nout ? __ldg(p.bias + o + e) : 0.0f;
+            return make_float4(b[0], b[1], b[2], b[3]);
+        };
+        if (pair < tiles) bias128[lane] = bias4(pair);
         drk_dep_wait();
         int slot = 0, at_ring = 0;
         uint32_t sphase = 0;
@@ -789,18 +802,48 @@ k_fp8_pair(const __grid_constant__ CUtensorMap mapW, const __grid_constant__ CUt
                 for (int j = 0; j < 8; j++)
                     reinterpret_cast<unsigned long long *>(stg)[lane * 8 + (j ^ (lane >> 1 & 7))] = acc[decltype(chunk)::value * 8 + j];
             };
-            float bias[4], next[4];
-            auto ask = [&](int o) {
+            /* 16-bit results are rounded first and leave 32 outputs at a time */
+            auto out16 = [&](auto two) {
+                using W = decltype(two);
+                auto stage32 = [&](auto chunk) {
+                    constexpr int c = decltype(chunk)::value;
 #pragma unroll
-                for (int e = 0; e < 4; e++) next[e] = p.bias && o + e < p.Nout ? __ldg(p.bias + o + e) : 0.0f;
+                    for (int j = 0; j < 8; j++) {
+                        const float4 b = bias128[c * 8 + j];
+                        const unsigned long long lo = acc[c * 16 + 2 * j], hi = acc[c * 16 + 2 * j + 1];
+                        const W w0 = fp8_store2<W>(fp8_act(__uint_as_float((uint32_t)lo) + b.x, p.act), fp8_act(__uint_as_float((uint32_t)(lo >> 32)) + b.y, p.act));
+                        const W w1 = fp8_store2<W>(fp8_act(__uint_as_float((uint32_t)hi) + b.z, p.act), fp8_act(__uint_as_float((uint32_t)(hi >> 32)) + b.w, p.act));
+                        reinterpret_cast<uint2 *>(stg)[lane * 8 + (j ^ (lane >> 1 & 7))] = make_uint2(reinterpret_cast<const uint32_t &>(w0), reinterpret_cast<const uint32_t &>(w1));
+                    }
+                };
+                const int left = p.n - row0 - (lane >> 2);
+                char *to = static_cast<char *>(p.out) + ((size_t)(row0 + (lane >> 2)) * p.ldo + ot * FP8_BLOCK + (lane & 3) * 8) * 2;
+                const size_t down = (size_t)p.ldo * 16;
+#pragma unroll 1
+                for (int c = 0; c < 4; c++, to += 64) {
+                    __syncwarp();
+                    if (c == 0) stage32(std::integral_constant<int, 0>{});
+                    else if (c == 1) stage32(std::integral_constant<int, 1>{});
+                    else if (c == 2) stage32(std::integral_constant<int, 2>{});
+                    else stage32(std::integral_constant<int, 3>{});
+                    __syncwarp();
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const int rr = i * 8 + (lane >> 2);
+                        uint4 w = reinterpret_cast<const uint4 *>(stg)[rr * 4 + ((lane & 3) ^ (rr >> 2 & 3))];
+                        if (rr >> 1 & 1) w = make_uint4(w.z, w.w, w.x, w.y);
+                        if (i * 8 < left) *reinterpret_cast<uint4 *>(to + i * down) = w;
+                    }
+                }
             };
-            ask(o0);
+            const float4 next_bias = bias4(min(t + pairs, tiles - 1));
+            if (vec && p.out_type != DRK_F32 && (ot + 1) * FP8_BLOCK <= p.Nout) {
+                if (p.out_type == DRK_BF16) out16(__nv_bfloat162());
+                else out16(__half2());
+            } else
 #pragma unroll 1
             for (int c = 0; c < 8; c++) {
                 const int o = o0 + c * 16;
-#pragma unroll
-                for (int e = 0; e < 4; e++) bias[e] = next[e];
-                if (c < 7) ask(o + 16);
                 __syncwarp();
                 switch (c) {
                 case 0: stage16(std::integral_constant<int, 0>{}); break;
@@ -813,14 +856,15 @@ k_fp8_pair(const __grid_constant__ CUtensorMap mapW, const __grid_constant__ CUt
                 default: stage16(std::integral_constant<int, 7>{}); break;
                 }
                 __syncwarp();
+                const float4 bias = bias128[c * 4 + (lane & 3)];
                 float v[4][4];
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                     const int rr = i * 8 + (lane >> 2);
                     float4 w = reinterpret_cast<const float4 *>(stg)[rr * 4 + ((lane & 3) ^ (rr >> 2 & 3))];
                     if (rr >> 1 & 1) w = make_float4(w.z, w.w, w.x, w.y);
-                    v[i][0] = fp8_act(w.x + bias[0], p.act); v[i][1] = fp8_act(w.y + bias[1], p.act);
-                    v[i][2] = fp8_act(w.z + bias[2], p.act); v[i][3] = fp8_act(w.w + bias[3], p.act);
+                    v[i][0] = fp8_act(w.x + bias.x, p.act); v[i][1] = fp8_act(w.y + bias.y, p.act);
+                    v[i][2] = fp8_act(w.z + bias.z, p.act); v[i][3] = fp8_act(w.w + bias.w, p.act);
                 }
                 const int left = p.n - row0 - (lane >> 2);      /* rows i * 8 below it exist */
                 const size_t at0 = (size_t)(row0 + (lane >> 2)) * p.ldo + o;
@@ -849,6 +893,8 @@ k_fp8_pair(const __grid_constant__ CUtensorMap mapW, const __grid_constant__ CUt
                     }
                 }
             }
+            __syncwarp();
+            bias128[lane] = next_bias;
         }
     }
     drk_dep_trigger();
