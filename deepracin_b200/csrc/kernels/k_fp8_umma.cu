@@ -382,7 +382,7 @@ k_fp8_swap(const __grid_constant__ CUtensorMap mapW, const __grid_constant__ CUt
         drk_dep_wait();
         auto rounding = [&](auto fast) {
             constexpr bool FAST = decltype(fast)::value;    /* whole vectors: the next block's are on their way while one is rounded */
-            const char *row[FUSE_ROWS];
+            const char *row[FUSE_ROWS] = {};
             Raw raw[FUSE_ROWS];
             float sw = 0.0f;
             auto fetch = [&](int b, int r) {
@@ -932,13 +932,13 @@ int drk_fp8_tensor_plan(Fp8Tensor *t, const Fp8Params *p, const void *codes, con
     t->split = 1;
     while (t->split < 8 && tiles * t->split * 2 <= room && t->split * 4 <= p->kb) t->split *= 2;
     t->stages = (p->kb + t->split - 1) / t->split;
-    /* Above 64 rows a block of 128 inputs takes a CTA of k_fp8_swap<128> 0.6 us and a pair of k_fp8_pair, on four times the tile,
-       0.4 us, and the pair starts 1 us later (4096 -> 4096: 256 rows 20 against 26 us, 384 rows 32 against 26 us; 8192 -> 8192,
-       256 rows: 50 against 37 us).  Rounds times blocks decide. */
+    /* Above 64 rows.  In units of 0.1 us a block of 128 inputs takes a CTA of k_fp8_swap<128> 5 and a pair of k_fp8_pair, on four
+       times the tile, 4; a round adds 10 to either, and the pair starts 10 later (4096 -> 4096: 256 rows 16.6 against 20.8 us, 600
+       rows 39.8 against 22.2 us; 1024 -> 4096, 256 rows: 10.2 against 11.8 us). */
     t->mtiles = (p->n + 255) / 256;
     t->ntiles = (p->ob + 1) / 2;
     const long long ptiles = (long long)t->mtiles * t->ntiles, rounds = ((long long)tiles * t->split + sms - 1) / sms, prounds = (ptiles + sms / 2 - 1) / (sms / 2);
-    t->pairs = p->n > 64 && 2 * prounds * p->kb + 5 <= 3 * rounds * t->stages ? (int)(ptiles < sms / 2 ? ptiles : sms / 2) : 0;
+    t->pairs = p->n > 64 && prounds * (4 * p->kb + 10) + 10 <= rounds * (5 * t->stages + 10) ? (int)(ptiles < sms / 2 ? ptiles : sms / 2) : 0;
     /* rounding inside the product's kernel costs nothing while its four warps keep up with the weights: 16-bit rows, one row, or a
        short share (25088 -> 4096, fp32: one row 19.8 against 22.2 us, two rows 23.8 against 22.4; 4096 -> 4096, four rows 7.6
        against 8.2) */
