@@ -125,6 +125,21 @@ def test_against_the_definition(n, nin, nout, types):
     check(layer.result(), quantized(x), dequantized(codes, scales), bias, act, -(-nin // 128))
 
 
+@pytest.mark.parametrize("tout", [F32, BF16, F16])
+@pytest.mark.parametrize("n,nin,nout,ldo", [(2501, 300, 8200, 8200), (2501, 300, 8200, 8204), (3001, 128, 5000, 5008), (2050, 257, 9001, 9001), (4001, 256, 256, 256), (900, 128, 1027, 1032)])
+def test_bias_and_activation_of_many_tiles(n, nin, nout, ldo, tout):
+    """several tiles for each pair of CTAs, whose bias is fetched a tile ahead; rows that can be stored 16 bytes at a time and others"""
+    g = torch.Generator().manual_seed(n + ldo)
+    x = torch.randn(n, nin, generator=g).cuda()
+    codes, scales = make_weights(nin, nout, 21)
+    scales = scales * 0.02
+    bias = torch.randn(nout, generator=g).cuda()
+    layer = Layer(x, codes, scales, bias, tout, 1, F32, ldo=ldo)
+    layer.run()
+    check(layer.result(), quantized(x), dequantized(codes, scales), bias, 1, -(-nin // 128))
+    assert bool((layer.out[:, nout:] == -77.0).all())
+
+
 @pytest.mark.parametrize("n,nin,nout", [(1, 700, 300), (37, 1003, 517), (300, 520, 389), (1100, 650, 1300), (1500, 1290, 2301)])
 @pytest.mark.parametrize("tin,tout", [(F32, F32), (BF16, F16)])
 def test_pitches_and_alignment(n, nin, nout, tin, tout):
