@@ -165,7 +165,9 @@ __device__ __forceinline__ bool mbar_wait1(uint32_t bar, uint32_t parity, volati
  *
  * Bound by the weights' way from HBM behind 4 us of launch, first loads and exchange: 1 x 25088 -> 4096 fp32 19.8 us (15.7 at the
  * copy rate), 1 x 4096 -> 4096 6.1 us (2.6); with 64 rows by the sums of a block too, and the rounding's launch: 64 x 25088 -> 4096
- * 25.1 us (16.8), 64 x 4096 -> 1000 8.1 us; with NT = 128 by the sums, 0.6 us a block.
+ * 24.5 us (16.8), 64 x 4096 -> 1000 7.8 us; with NT = 128 by the sums, 0.6 us a block, and 5 us of start and end, where code runs
+ * once and costs its way from the L2 (4000 x 256 -> 256 bf16: 8.0 us with the rounding, 15.7 us when an unsplit tile's results
+ * went through the inbox row by row).
  *
  * FUSE (the bytes of an input value; at most FUSE_ROWS rows): four more warps round the input themselves, a block each in turn,
  * straight into the swizzled operand tile; what takes two launches takes one.
@@ -524,12 +526,16 @@ k_fp8_swap(const __grid_constant__ CUtensorMap mapW, const __grid_constant__ CUt
  * makes the factors sx * sw of a block and leaves them in shared memory.
  *
  * What bounds it: the way issue -> commit -> read -> hand back -> issue, 700 to 900 clocks a block with two accumulators under
- * way, where the MMAs take 512; in a long run the board's power (half of it spent on copies and at rest, a third on the MMAs).
- * 4096 x 8192 -> 8192 with the rounding of the input: 270 us alone, 316 us back to back (980 W, 1.55 GHz; 8 row tiles walked
- * together instead of 16: 321 us); copies and MMAs without the sums 207 us.  Measured on the way there (back to back): factors read by the summing warps themselves 341 us (the instructions
- * that ran once in four blocks stalled each time, those of a loop unrolled by two or four missed the instruction cache: 384 us),
- * scalar FMAs 337 us, one issuing warp 328 us, sixteen summing warps 409 us; a cluster-scope release on the hand-back (a memory
- * barrier) and registers copied after a separate wait cost 100 us and more each.
+ * way, where the MMAs take 512; 8 us of start (registers, TMEM, barriers of two CTAs, first loads: 3) and of a tile's results
+ * (10000 clocks each when every chunk had code of its own, bank conflicts and its bias to wait for); in a long run the board's
+ * power (half of it spent on copies and at rest, a third on the MMAs).  With the rounding of the input, 4096 x 8192 -> 8192 bf16:
+ * 256 us alone, 296 us back to back (980 W, 1.45 to 1.55 GHz), copies and MMAs without the sums 207 us; 1000 x 4096 -> 4096 23.9 us.
+ * Measured on the way there (back to back): factors read by the summing warps themselves 341 us (the instructions that ran once
+ * in four blocks stalled each time, those of a loop unrolled by two or four missed the instruction cache: 384 us), scalar FMAs
+ * 337 us, one issuing warp 328 us, sixteen summing warps 409 us, 8 row tiles walked together instead of 16 321 us, these against
+ * 316 us; a cluster-scope release on the hand-back (a memory barrier) and registers copied after a separate wait cost 100 us and
+ * more each, and so do a few registers more in the results' code (335 us: the sums are spilled), or sums staged in fours, which
+ * wants them in aligned registers (338 us).
  */
 struct PairCfg {
     static constexpr int STAGE_BYTES = 2 * FP8_BLOCK_BYTES;

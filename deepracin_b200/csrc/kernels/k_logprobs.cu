@@ -222,8 +222,7 @@ __global__ void __launch_bounds__(LP_WNT) k_logprobs_short(const LpParams p, con
     __shared__ uint16_t items[LP_WNT / 32][32 * U];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const size_t row = (size_t)blockIdx.x * (LP_WNT / 32) + warp;
-    drk_dep_wait();
-    drk_dep_trigger();
+    drk_dep_wait();     /* no trigger: see k_logprobs (2000 x 1000 fp32, k = 20: 6.9 instead of 5.7 us) */
     if (row >= (size_t)n) return;
     const T *v = static_cast<const T *>(p.logits) + row * p.ld;
     const int head = min(p.len, (int)((16 - (uintptr_t)v % 16) % 16 / sizeof(T)));
