@@ -948,20 +948,51 @@ static int encode_rows(CUtensorMap *map, const void *base, size_t rows, int box_
                                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS ? 0 : -1;
 }
 
+/* how many clusters of `split` CTAs that have an SM to themselves run at once: fewer than sms / split, as a cluster stays inside one
+ * of the GPU's groups of SMs (33 of four, 15 of eight) */
+static int swap_clusters(int split, int sms)
+{
+    if (split == 1) return sms;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)split);
+    cfg.blockDim = dim3(SwapCfg<16, 0>::THREADS);
+    cfg.dynamicSmemBytes = SwapCfg<16, 0>::smem(SwapCfg<16, 0>::STAGES);
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = (unsigned)split;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    int n = 0;
+    if (cudaFuncSetAttribute(k_fp8_swap<16, 0>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)cfg.dynamicSmemBytes) != cudaSuccess ||
+        cudaOccupancyMaxActiveClusters(&n, k_fp8_swap<16, 0>, &cfg) != cudaSuccess) {
+        (void)cudaGetLastError();
+        return sms / split * 3 / 4;
+    }
+    return n < sms / split ? n : sms / split;
+}
+
 int drk_fp8_tensor_plan(Fp8Tensor *t, const Fp8Params *p, const void *codes, const void *q, int sms)
 {
     t->nt = p->n <= 16 ? 16 : p->n <= 32 ? 32 : p->n <= 64 ? 64 : 128;
-    /* as many shares of a tile's blocks as still run at once, one on an SM */
-    const int tiles = p->ob * ((p->n + t->nt - 1) / t->nt), room = sms;
+    /* as many shares of a tile's blocks as still run at once, one on an SM (64 x 4096 -> 2304: 18 clusters of eight, of which 15 fit,
+       14.3 us, of four 9.3 us) */
+    const int tiles = p->ob * ((p->n + t->nt - 1) / t->nt);
+    int at_once = sms;
     t->split = 1;
-    while (t->split < 8 && tiles * t->split * 2 <= room && t->split * 4 <= p->kb) t->split *= 2;
+    while (t->split < 8 && t->split * 4 <= p->kb && tiles * t->split * 2 <= sms) {
+        const int clusters = swap_clusters(t->split * 2, sms);
+        if (tiles > clusters) break;
+        t->split *= 2;
+        at_once = clusters;
+    }
     t->stages = (p->kb + t->split - 1) / t->split;
     /* Above 64 rows.  In units of 0.1 us a block of 128 inputs takes a CTA of k_fp8_swap<128> 5 and a pair of k_fp8_pair, on four
        times the tile, 4; a round adds 10 to either, and the pair starts 10 later (4096 -> 4096: 256 rows 16.6 against 20.8 us, 600
        rows 39.8 against 22.2 us; 1024 -> 4096, 256 rows: 10.2 against 11.8 us). */
     t->mtiles = (p->n + 255) / 256;
     t->ntiles = (p->ob + 1) / 2;
-    const long long ptiles = (long long)t->mtiles * t->ntiles, rounds = ((long long)tiles * t->split + sms - 1) / sms, prounds = (ptiles + sms / 2 - 1) / (sms / 2);
+    const long long ptiles = (long long)t->mtiles * t->ntiles, rounds = ((long long)tiles + at_once - 1) / at_once, prounds = (ptiles + sms / 2 - 1) / (sms / 2);
     t->pairs = p->n > 64 && prounds * (4 * p->kb + 10) + 10 <= rounds * (5 * t->stages + 10) ? (int)(ptiles < sms / 2 ? ptiles : sms / 2) : 0;
     /* rounding inside the product's kernel costs nothing while its four warps keep up with the weights: 16-bit rows, one row, or a
        short share (25088 -> 4096, fp32: one row 19.8 against 22.2 us, two rows 23.8 against 22.4; 4096 -> 4096, four rows 7.6

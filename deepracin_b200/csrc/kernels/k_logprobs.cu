@@ -218,7 +218,7 @@ __global__ void __launch_bounds__(LP_WNT) k_logprobs_short(const LpParams p, con
     using Y = LpType<T>;
     constexpr int V = Y::V;
     __shared__ __align__(16) unsigned long long cands[LP_WNT / 32][LP_WCAND + 2], lists[LP_WNT / 32][LP_KMAX];
-    __shared__ __align__(16) uint32_t lanes[LP_WNT / 32][32];
+    __shared__ __align__(16) uint32_t lanes[LP_WNT / 32][64];
     __shared__ uint16_t items[LP_WNT / 32][32 * U];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const size_t row = (size_t)blockIdx.x * (LP_WNT / 32) + warp;
@@ -275,16 +275,39 @@ __global__ void __launch_bounds__(LP_WNT) k_logprobs_short(const LpParams p, con
     for (int o = 16; o > 0; o >>= 1) { S += __shfl_xor_sync(0xffffffffu, S, o); E += __shfl_xor_sync(0xffffffffu, E, o); }
 
     if (p.k > 0) {
-        lanes[warp][lane] = own;
-        __syncwarp();
-        int r = 0;
+        uint32_t border;
+        if (p.k <= 24) {
+            lanes[warp][lane] = own;
+            __syncwarp();
+            int r = 0;
 #pragma unroll
-        for (int j = 0; j < 32; j += 4) {
-            const uint4 y = *reinterpret_cast<const uint4 *>(&lanes[warp][j]);
-            r += (y.x > own || (y.x == own && j < lane)) + (y.y > own || (y.y == own && j + 1 < lane)) + (y.z > own || (y.z == own && j + 2 < lane)) +
-                 (y.w > own || (y.w == own && j + 3 < lane));
+            for (int j = 0; j < 32; j += 4) {
+                const uint4 y = *reinterpret_cast<const uint4 *>(&lanes[warp][j]);
+                r += (y.x > own || (y.x == own && j < lane)) + (y.y > own || (y.y == own && j + 1 < lane)) + (y.z > own || (y.z == own && j + 2 < lane)) +
+                     (y.w > own || (y.w == own && j + 3 < lane));
+            }
+            border = __shfl_sync(0xffffffffu, own, __ffs(__ballot_sync(0xffffffffu, r == p.k - 1)) - 1);
+        } else {
+            /* two parts of a lane's share: the k-th largest of 64 maxima, which 44 values are expected to reach at k = 32 (130 reach
+               the least of 32, and at times more than a warp ranks: 20000 x 1000 fp32, k = 32: 50 instead of 125 us, k = 28: 48
+               instead of 49; at k = 24 42 instead of 38) */
+            float a0 = -INFINITY, a1 = -INFINITY;
+#pragma unroll
+            for (int u = 0; u < U; u += 2) { a0 = lp_max_nan(a0, vm[u]); a1 = lp_max_nan(a1, vm[u + 1]); }
+            const uint32_t g0 = max(lane < nvec ? lp_order(a0) : 0u, lane < singles ? lp_order(alone) : 0u), g1 = 32 + lane < nvec ? lp_order(a1) : 0u;
+            lanes[warp][lane] = g0;
+            lanes[warp][32 + lane] = g1;
+            __syncwarp();
+            int r0 = 0, r1 = 0;
+#pragma unroll 4
+            for (int j = 0; j < 64; j++) {
+                const uint32_t y = lanes[warp][j];
+                r0 += y > g0 || (y == g0 && j < lane);
+                r1 += y > g1 || (y == g1 && j < 32 + lane);
+            }
+            const uint32_t mine0 = __ballot_sync(0xffffffffu, r0 == p.k - 1), mine1 = __ballot_sync(0xffffffffu, r1 == p.k - 1);
+            border = __shfl_sync(0xffffffffu, mine0 ? g0 : g1, __ffs(mine0 | mine1) - 1);
         }
-        const uint32_t border = __shfl_sync(0xffffffffu, own, __ffs(__ballot_sync(0xffffffffu, r == p.k - 1)) - 1);
         const float low = lp_value(border);         /* NaN where everything counts */
         const uint32_t before = (1u << lane) - 1;
         int count = 0, found = 0;
