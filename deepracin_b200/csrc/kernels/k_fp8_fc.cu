@@ -43,79 +43,67 @@ template <typename T> __device__ __forceinline__ float fp8_largest(const uint4 *
 }
 
 /* ------------------------------------------------------------------ activations
- * A half warp owns a block of 128 values of one row, 8 per lane, and asks for U blocks before it rounds the first; each lane
- * divides for one of them.  Bound by HBM in 32 bits (reads sizeof(T), writes one byte a value; 4096 x 8192: 27 us, 26 at the copy
- * rate), in 16 bits by the issue too (22 us, 15 at the copy rate; 24 us with every lane dividing for all and a division for each
- * block's place).  U = 1: 30 us in 16 bits, U = 4: 22 us, U = 8: 25 us.
+ * A team of 16 / G lanes owns a block of 128 values of one row, G times 8 per lane.  Bound by HBM (reads sizeof(T), writes one byte
+ * a value; 4096 x 8192: fp32 28 us, 26 at the copy rate; bf16 17.4 us, 15) when G = 2; with G = 1 a warp issues nearly twice as
+ * much per value (bf16 21.6 us), G = 4 is no faster and twice as slow off 16-byte boundaries.  Few blocks: G = 1, more warps.
  * q: [block][n rows][128], sx: [block][n rows]. */
-template <typename T, int U>
+template <typename T, int G>
 __global__ void __launch_bounds__(256) k_fp8_quantize_rows(const T *__restrict__ in, size_t ldi, unsigned char *__restrict__ q, float *__restrict__ sx,
                                                            int n, int Nin, int kb, int vec)
 {
     drk_dep_wait();
     drk_dep_trigger();
     constexpr int W = sizeof(T) / 2;        /* 16-byte loads of 8 values */
-    const int sub = threadIdx.x & 15;
-    const unsigned total = (unsigned)n * (unsigned)kb, halves = gridDim.x * (blockDim.x / 16);
-    /* whole warps stay in the loop: both halves shuffle together */
-    unsigned i0 = blockIdx.x * (blockDim.x / 16) + (threadIdx.x >> 5) * 2;
-    const unsigned first = i0 + ((threadIdx.x >> 4) & 1), drow = halves / (unsigned)kb, dblk = halves - drow * (unsigned)kb;
+    constexpr int LANES = 16 / G, TEAMS = 32 / LANES;
+    const int sub = threadIdx.x % LANES;
+    const unsigned total = (unsigned)n * (unsigned)kb, teams = gridDim.x * (blockDim.x / LANES);
+    /* whole warps stay in the loop: their teams shuffle together */
+    unsigned i0 = (blockIdx.x * (blockDim.x / 32) + (threadIdx.x >> 5)) * TEAMS;
+    const unsigned first = i0 + (threadIdx.x & 31) / LANES, drow = teams / (unsigned)kb, dblk = teams - drow * (unsigned)kb;
     unsigned row = first / (unsigned)kb, blk = first - row * (unsigned)kb;
-    for (; i0 < total; i0 += U * halves) {
-        uint4 raw[U][W];
-        unsigned rows[U], blks[U];
-        float a[U];
+    for (; i0 < total; i0 += teams) {
+        const bool here = row < (unsigned)n;
+        uint4 raw[G][W];
+        float a = FP8_FLOOR;
 #pragma unroll
-        for (int u = 0; u < U; u++) {
-            rows[u] = row; blks[u] = blk;
-            const int k0 = (int)blk * FP8_BLOCK + sub * 8;
+        for (int g = 0; g < G; g++) {
+            const int k0 = (int)blk * FP8_BLOCK + (g * LANES + sub) * 8;
             const T *src = in + row * ldi + k0;
 #pragma unroll
-            for (int j = 0; j < W; j++) raw[u][j] = make_uint4(0u, 0u, 0u, 0u);
-            if (row < (unsigned)n) {
-                if (vec && k0 + 8 <= Nin) {
+            for (int j = 0; j < W; j++) raw[g][j] = make_uint4(0u, 0u, 0u, 0u);
+            if (here && vec && k0 + 8 <= Nin) {
 #pragma unroll
-                    for (int j = 0; j < W; j++) raw[u][j] = __ldg(reinterpret_cast<const uint4 *>(src) + j);
-                } else {
-                    T *one = reinterpret_cast<T *>(raw[u]);
+                for (int j = 0; j < W; j++) raw[g][j] = __ldg(reinterpret_cast<const uint4 *>(src) + j);
+            } else if (here) {
+                T *one = reinterpret_cast<T *>(raw[g]);
 #pragma unroll
-                    for (int j = 0; j < 8; j++) if (k0 + j < Nin) one[j] = src[j];
-                }
+                for (int j = 0; j < 8; j++) if (k0 + j < Nin) one[j] = src[j];
             }
-            row += drow;
-            blk += dblk;
-            if (blk >= (unsigned)kb) { blk -= kb; row++; }
         }
 #pragma unroll
-        for (int u = 0; u < U; u++) a[u] = fmaxf(FP8_FLOOR, fp8_largest<T>(raw[u]));
+        for (int g = 0; g < G; g++) a = fmaxf(a, fp8_largest<T>(raw[g]));
 #pragma unroll
-        for (int o = 8; o > 0; o >>= 1)
+        for (int o = LANES / 2; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o));
+        const float inv = __fdiv_rn(FP8_MAX, a), scale = __fdiv_rn(a, FP8_MAX);
+        const size_t at = (size_t)blk * n + row;
 #pragma unroll
-            for (int u = 0; u < U; u++) a[u] = fmaxf(a[u], __shfl_xor_sync(0xffffffffu, a[u], o));
-        /* a lane divides for one of the U blocks */
-        float b = a[0];
-#pragma unroll
-        for (int u = 1; u < U; u++) b = sub % U == u ? a[u] : b;
-        const float bi = __fdiv_rn(FP8_MAX, b), bs = __fdiv_rn(b, FP8_MAX);
-#pragma unroll
-        for (int u = 0; u < U; u++) {
-            const float inv = U == 1 ? bi : __shfl_sync(0xffffffffu, bi, u, 16);
+        for (int g = 0; g < G; g++) {
             float v[8];
             uint32_t c[2];
 #pragma unroll
-            for (int j = 0; j < 8; j++) v[j] = fp8_load(reinterpret_cast<const T *>(raw[u]) + j) * inv;
+            for (int j = 0; j < 8; j++) v[j] = fp8_load(reinterpret_cast<const T *>(raw[g]) + j) * inv;
 #pragma unroll
             for (int j = 0; j < 2; j++) {
                 const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(v[4 * j], v[4 * j + 1]), __NV_SATFINITE, __NV_E4M3);
                 const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(v[4 * j + 2], v[4 * j + 3]), __NV_SATFINITE, __NV_E4M3);
                 c[j] = lo | (hi << 16);
             }
-            if (rows[u] < (unsigned)n) {
-                const size_t at = (size_t)blks[u] * n + rows[u];
-                *reinterpret_cast<uint2 *>(q + at * FP8_BLOCK + sub * 8) = make_uint2(c[0], c[1]);
-                if (sub == u) sx[at] = bs;
-            }
+            if (here) *reinterpret_cast<uint2 *>(q + at * FP8_BLOCK + (g * LANES + sub) * 8) = make_uint2(c[0], c[1]);
         }
+        if (here && sub == 0) sx[at] = scale;
+        row += drow;
+        blk += dblk;
+        if (blk >= (unsigned)kb) { blk -= kb; row++; }
     }
 }
 
@@ -314,12 +302,11 @@ extern "C" dRk_Fp8FcPlan *dRk_fp8_fc_plan(const void *in, int in_type, long long
 
 template <typename T> static int fp8_quantize(const dRk_Fp8FcPlan *p, cudaStream_t st)
 {
-    /* few blocks: one for each half warp; many: two under way in each, eight CTAs to an SM */
-    const size_t halves = (size_t)p->p.n * p->p.kb;
-    const bool many = halves > 4 * 16 * 148 * 4;
-    const unsigned blocks = drk_blocks(many ? (halves + 1) / 2 : halves, 16, 148u * 8u);
-    return drk_launched(drk_launch_dep(many ? k_fp8_quantize_rows<T, 2> : k_fp8_quantize_rows<T, 1>, dim3(blocks), dim3(256), 0, st, (const T *)p->p.in,
-                                       p->p.ldi, p->q, p->sx, p->p.n, p->p.Nin, p->p.kb, p->p.vec));
+    /* many: more blocks than half warps find a place for (eight CTAs on an SM) */
+    const size_t blocks = (size_t)p->p.n * p->p.kb;
+    const bool many = blocks > 16 * 148 * 8;
+    return drk_launched(drk_launch_dep(many ? k_fp8_quantize_rows<T, 2> : k_fp8_quantize_rows<T, 1>, dim3(drk_blocks(blocks, many ? 32 : 16, 148u * 8u)), dim3(256), 0, st,
+                                       (const T *)p->p.in, p->p.ldi, p->q, p->sx, p->p.n, p->p.Nin, p->p.kb, p->p.vec));
 }
 
 extern "C" int dRk_fp8_fc_run(dRk_stream stream, dRk_Fp8FcPlan *p)
