@@ -529,7 +529,7 @@ k_fp8_swap(const __grid_constant__ CUtensorMap mapW, const __grid_constant__ CUt
  * way, where the MMAs take 512; 8 us of start (registers, TMEM, barriers of two CTAs, first loads: 3) and of a tile's results
  * (10000 clocks each when every chunk had code of its own, bank conflicts and its bias to wait for); in a long run the board's
  * power (half of it spent on copies and at rest, a third on the MMAs).  With the rounding of the input, 4096 x 8192 -> 8192 bf16:
- * 256 us alone, 296 us back to back (980 W, 1.45 to 1.55 GHz), copies and MMAs without the sums 207 us; 1000 x 4096 -> 4096 23.9 us.
+ * 249 us alone, 292 us back to back (980 W, 1.43 GHz), copies and MMAs without the sums 207 us; 1000 x 4096 -> 4096 23.1 us.
  * Measured on the way there (back to back): factors read by the summing warps themselves 341 us (the instructions that ran once
  * in four blocks stalled each time, those of a loop unrolled by two or four missed the instruction cache: 384 us), scalar FMAs
  * 337 us, one issuing warp 328 us, sixteen summing warps 409 us, 8 row tiles walked together instead of 16 321 us, these against
