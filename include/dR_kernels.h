@@ -248,7 +248,7 @@ enum { DRK_F32 = 0, DRK_BF16 = 1, DRK_F16 = 2 };
  * A row that holds an infinity or a NaN becomes NaN; the other rows do not see it.
  * A plan keeps the pointers it was made with and belongs to the device that was current; run refuses another one, or another
  * device's stream (-6).  Runs of plans that share a scratch or an output must not overlap on the GPU; neither must two runs of
- * one plan on two streams.  A run only enqueues (two launches), allocates nothing and may be captured into a CUDA graph.
+ * one plan on two streams.  A run only enqueues (one or two launches), allocates nothing and may be captured into a CUDA graph.
  * The packed weights are read ahead of the launch in front: write them with the calls below, copies, or kernels without an early
  * programmatic trigger.  `status` (may be NULL) as dRk_tensor_conv_plan.  _plan returns NULL, the others a negative value, with a message on stderr,
  * for arguments that they refuse.
