@@ -972,13 +972,13 @@ static int swap_clusters(int split, int sms)
     return n < sms / split ? n : sms / split;
 }
 
-int drk_fp8_tensor_plan(Fp8Tensor *t, const Fp8Params *p, const void *codes, const void *q, int sms)
+/* shares of a tile's blocks in k_fp8_swap<nt>: as many as still run at once, one on an SM (64 x 4096 -> 2304: 18 clusters of eight,
+ * of which 15 fit, 14.3 us, of four 9.3 us); returns the rounds */
+static long long swap_split(Fp8Tensor *t, const Fp8Params *p, int nt, int sms)
 {
-    t->nt = p->n <= 16 ? 16 : p->n <= 32 ? 32 : p->n <= 64 ? 64 : 128;
-    /* as many shares of a tile's blocks as still run at once, one on an SM (64 x 4096 -> 2304: 18 clusters of eight, of which 15 fit,
-       14.3 us, of four 9.3 us) */
-    const int tiles = p->ob * ((p->n + t->nt - 1) / t->nt);
+    const long long tiles = (long long)p->ob * ((p->n + nt - 1) / nt);
     int at_once = sms;
+    t->nt = nt;
     t->split = 1;
     while (t->split < 8 && t->split * 4 <= p->kb && tiles * t->split * 2 <= sms) {
         const int clusters = swap_clusters(t->split * 2, sms);
@@ -987,13 +987,28 @@ int drk_fp8_tensor_plan(Fp8Tensor *t, const Fp8Params *p, const void *codes, con
         at_once = clusters;
     }
     t->stages = (p->kb + t->split - 1) / t->split;
-    /* Above 64 rows.  In units of 0.1 us a block of 128 inputs takes a CTA of k_fp8_swap<128> 5 and a pair of k_fp8_pair, on four
-       times the tile, 4; a round adds 10 to either, and the pair starts 10 later (4096 -> 4096: 256 rows 16.6 against 20.8 us, 600
-       rows 39.8 against 22.2 us; 1024 -> 4096, 256 rows: 10.2 against 11.8 us). */
+    return (tiles + at_once - 1) / at_once;
+}
+
+int drk_fp8_tensor_plan(Fp8Tensor *t, const Fp8Params *p, const void *codes, const void *q, int sms)
+{
     t->mtiles = (p->n + 255) / 256;
     t->ntiles = (p->ob + 1) / 2;
-    const long long ptiles = (long long)t->mtiles * t->ntiles, rounds = ((long long)tiles + at_once - 1) / at_once, prounds = (ptiles + sms / 2 - 1) / (sms / 2);
-    t->pairs = p->n > 64 && prounds * (4 * p->kb + 10) + 10 <= rounds * (5 * t->stages + 10) ? (int)(ptiles < sms / 2 ? ptiles : sms / 2) : 0;
+    t->pairs = 0;
+    if (p->n <= 64) swap_split(t, p, p->n <= 16 ? 16 : p->n <= 32 ? 32 : 64, sms);
+    else {
+        /* In units of 0.05 us a block of 128 inputs takes a CTA of k_fp8_swap<64> 5, one of k_fp8_swap<128> 9, and a pair of
+           k_fp8_pair, on four times the latter's tile, 8; a round adds 30, 16 and 20, and the pair starts 10 later (fitted on 399
+           shapes, 0.5 % worse than the best of the three in each.  In this order, 4096 -> 3200: 17.7, 22.5 and 20.7 us for 300
+           rows; 18560 -> 1792: 31.0, 45.0 and 61.4; 4096 -> 7680, 700 rows: 74.0, 59.6 and 36.5). */
+        const long long ptiles = (long long)t->mtiles * t->ntiles, prounds = (ptiles + sms / 2 - 1) / (sms / 2);
+        long long rounds = swap_split(t, p, 64, sms);
+        const long long cost64 = rounds * (5 * t->stages + 30);
+        rounds = swap_split(t, p, 128, sms);
+        const long long cost128 = rounds * (9 * t->stages + 16), paired = prounds * (8 * p->kb + 20) + 10;
+        if (paired <= cost128 && paired <= cost64) t->pairs = (int)(ptiles < sms / 2 ? ptiles : sms / 2);
+        else if (cost64 < cost128) swap_split(t, p, 64, sms);
+    }
     /* rounding inside the product's kernel costs nothing while its four warps keep up with the weights: 16-bit rows, one row, or a
        short share (25088 -> 4096, fp32: one row 19.8 against 22.2 us, two rows 23.8 against 22.4; 4096 -> 4096, four rows 7.6
        against 8.2) */

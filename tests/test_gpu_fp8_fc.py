@@ -105,6 +105,8 @@ def check(got, xq, w, bias, act, kb):
 SHAPES = [(1, 1, 1), (1, 128, 128), (2, 129, 127), (3, 127, 257), (5, 16, 3), (16, 256, 384), (17, 1000, 100), (37, 1003, 517),
           (33, 2176, 1000), (64, 4096, 1000), (65, 640, 130), (96, 1500, 129), (128, 384, 256), (129, 300, 200), (200, 2049, 260),
           (256, 512, 512), (300, 1024, 640), (513, 256, 1000), (1000, 512, 300), (1, 25088, 384), (1030, 1290, 2060), (2500, 384, 515),
+          # several tiles of 64 rows, in shares and whole
+          (150, 8300, 300), (330, 5000, 1800), (70, 4100, 4500),
           # pairs of CTAs on 256 x 256 tiles: ragged edges, an odd number of weight blocks, one block, several tiles for each pair
           (129, 2000, 8200), (333, 3000, 4100), (1500, 1290, 2300), (2100, 900, 1100), (2500, 300, 8200), (3000, 100, 5000)]
 
