@@ -117,14 +117,6 @@ __device__ __forceinline__ void st_cluster(uint32_t cluster_addr, float v)
 {
     asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(cluster_addr), "f"(v) : "memory");
 }
-__device__ __forceinline__ void fp8_put(const Fp8Params &p, size_t r, int o, float v)
-{
-    v = fp8_act(v, p.act);
-    const size_t at = r * p.ldo + o;
-    if (p.out_type == DRK_F32) static_cast<float *>(p.out)[at] = v;
-    else if (p.out_type == DRK_BF16) static_cast<__nv_bfloat16 *>(p.out)[at] = fp8_store<__nv_bfloat16>(v);
-    else static_cast<__half *>(p.out)[at] = fp8_store<__half>(v);
-}
 
 /* a wait of a whole warp that holds many registers: no call inside, which would have them saved around it */
 __device__ __forceinline__ bool mbar_wait_warp_inline(uint32_t bar, uint32_t parity, volatile int *abort_flag, int *status, int code)

@@ -275,7 +275,8 @@ void dRk_fp8_fc_free(dRk_Fp8FcPlan *plan);
  *   entropy [n]         -sum p log p (natural logarithm); NULL: not wanted
  *   top_logprob, top_index [n][k]  the k <= min(32, len) largest logits, descending, equal ones by ascending index, NaN first
  * Logits of -inf have probability 0 (a mask); a row of nothing else scores -inf everywhere, its entropy is 0.  A NaN or +inf
- * makes every score of its row NaN (the order of the alternatives stands).  m = 0 and k = 0 are allowed.  Sums are held in 32 bits.  Next to dRk_softmax (src/dR_nodes_math.c:620-678), which writes the probabilities themselves.
+ * makes every score of its row NaN (the order of the alternatives stands).  m = 0 and k = 0 are allowed.  Sums are held in 32
+ * bits.  Next to dRk_softmax (src/dR_nodes_math.c:620-678), which writes the probabilities themselves.
  * At most 2^28 rows of 2^30 logits; 0 < scale <= 2^120.  One launch, no workspace; -1 (with a message on stderr) for refused arguments, -6 for another device's stream.
  */
 int dRk_logprobs(dRk_stream stream, const void *logits, int type, long long ld, int n, int len, float scale, const int *labels, int m,
