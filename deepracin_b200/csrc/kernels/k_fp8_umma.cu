@@ -106,7 +106,7 @@ __device__ __forceinline__ void cluster_wait()
     __syncwarp();
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-/* a store to this address in the shared memory of the cluster's CTA `rank` */
+/* where saddr lies in the shared memory of the cluster's CTA `rank` */
 __device__ __forceinline__ uint32_t cluster_addr(uint32_t saddr, uint32_t rank)
 {
     uint32_t a;
