@@ -163,6 +163,20 @@ def test_pitches_and_alignment(n, nin, nout, tin, tout):
     assert bool((out[:, nout:] == -77.0).all()) and float(oflat[0]) == -77.0
 
 
+@pytest.mark.parametrize("n,nin,ldi", [(700, 4099, 4099), (2600, 1025, 1027), (1200, 2050, 2051)])
+def test_many_rows_off_every_boundary(n, nin, ldi):
+    g = torch.Generator().manual_seed(nin)
+    flat = torch.full((n * ldi + 1,), float("nan"), device="cuda")
+    view = flat[1:].view(n, ldi)
+    x = (torch.randn(n, nin, generator=g) * (0.25 + torch.rand(n, 1, generator=g))).cuda()
+    x[5] = 0
+    view[:, :nin] = x
+    codes, scales = make_weights(nin, 130, 8)
+    layer = Layer(x, codes, scales, None, F32, 0, F32, ldi=ldi, xptr=view.data_ptr())
+    layer.run()
+    check(layer.result(), quantized(x), dequantized(codes, scales), None, 0, -(-nin // 128))
+
+
 def test_codes_with_a_row_pitch_and_packing_of_the_float_matrix():
     lib = _lib()
     nin, nout = 333, 259
